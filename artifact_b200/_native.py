@@ -68,6 +68,10 @@ class PlanInfo(ctypes.Structure):
         "num_tiles", "tile_items", "tile_entries", "tile_shared_entries", "tile_staged_rows")]
 
 
+class Dropout(ctypes.Structure):
+    _fields_ = [("p", c_double), ("seed", c_uint64), ("step", c_uint64), ("step_dev", c_void_p), ("first_row", c_int64)]
+
+
 # every symbol include/rof_b200.h declares: (name, restype, argtypes)
 CUDA_ABI = [
     ("rof_plan_create_parts", c_int, [ctypes.POINTER(c_void_p), c_int, c_int, c_int, c_int, c_void_p, c_int64,
@@ -101,6 +105,17 @@ CUDA_ABI = [
     ("rof_shared_open", c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     ("rof_shared_close", c_int, [c_void_p]),
     ("rof_shared_free", c_int, [c_void_p]),
+    ("rof_layer_norm_workspace_bytes", c_int64, [c_int64, c_int]),
+    ("rof_layer_norm_forward", c_int, [c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,
+                                       ctypes.c_float, c_int, ctypes.POINTER(Dropout), c_void_p, c_int64, c_void_p,
+                                       c_void_p]),
+    ("rof_layer_norm_backward", c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p,
+                                        c_void_p, c_void_p, c_int, ctypes.POINTER(Dropout), c_void_p, c_int64, c_void_p,
+                                        c_void_p, c_void_p, c_int64, c_void_p]),
+    ("rof_dropout_forward", c_int, [c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int,
+                                    ctypes.POINTER(Dropout), c_void_p, c_int64, c_void_p]),
+    ("rof_dropout_backward", c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
+                                     ctypes.POINTER(Dropout), c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     ("rof_plan_take_status", c_int, [c_void_p]),
     ("rof_last_launch_count", c_int, []),
     ("rof_last_error", c_char_p, []),

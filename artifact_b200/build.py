@@ -19,7 +19,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "_lib")
 INCLUDE = os.path.join(ROOT, "include")
 
-CUDA_SOURCES = ["plan.cu", "kernels.cu", "api.cu", "stages.cu", "static_scratch.cu"]
+CUDA_SOURCES = ["plan.cu", "kernels.cu", "api.cu", "stages.cu", "static_scratch.cu", "norm.cu"]
 HOST_SOURCES = [os.path.join("host", "graphgen.cpp"), os.path.join("host", "reuse_search.cpp")]
 
 NVCC_FLAGS = [
@@ -67,7 +67,7 @@ def build_cuda(force=False, verbose=True, ptxas_info=False):
     target = cuda_lib_path()
     if not force and not _stale(target, srcs + hdrs + [os.path.abspath(__file__)]):
         return target
-    cmd = [_nvcc()] + NVCC_FLAGS + ["-I", INCLUDE, "-I", CSRC, "-shared", "-o", target] + srcs
+    cmd = [_nvcc(), "--threads", "0"] + NVCC_FLAGS + ["-I", INCLUDE, "-I", CSRC, "-shared", "-o", target] + srcs
     if ptxas_info:
         cmd += ["-Xptxas", "-v"]
     cmd += ["-lcudart", "-lgomp"]

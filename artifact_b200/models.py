@@ -6,6 +6,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from . import norm as N
 from .plan import AggregationPlan, scale_rows
 from .reuse_conv import ROF_GCNConv
 
@@ -75,29 +76,66 @@ class ROF_inputInfo:
 
 class ROF_GCN(torch.nn.Module):
     """n_layers hidden ROF_GCNConv layers + one output layer; activation and dropout between
-    layers (constructor keywords of ROF_main.py:192-200)."""
+    layers (constructor keywords of ROF_main.py:192-200).  Two keywords upstream does not have:
+    norm="layer" puts a layer norm in front of every activation; dropout_source="counter" draws the
+    dropout from the counter-based generator of norm.py (seed, step, row_offset of forward(); layer i of the stack takes
+    step + i * 2**40), in one pass with what stands before it when the activation is F.relu."""
 
     def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=F.relu, dropout=0.5, add_self_loops=False,
-                 reuse_size=0, kernel_type="ROF_v1", weight_initializer="glorot"):
+                 reuse_size=0, kernel_type="ROF_v1", weight_initializer="glorot", norm=None, dropout_source="torch"):
         super().__init__()
+        if norm not in (None, "layer") or dropout_source not in ("torch", "counter"):
+            raise ValueError("ROF_GCN: norm is None or 'layer', dropout_source 'torch' or 'counter'")
         kw = dict(add_self_loops=add_self_loops, reuse_size=reuse_size, kernel_type=kernel_type,
                   weight_initializer=weight_initializer)
         dims = [in_feats] + [n_hidden] * n_layers + [n_classes]
         self.layers = torch.nn.ModuleList(ROF_GCNConv(a, b, **kw) for a, b in zip(dims[:-1], dims[1:]))
-        self.activation, self.dropout = activation, dropout
+        self.activation, self.dropout, self.dropout_source = activation, dropout, dropout_source
+        # (not among the children without a norm: the state of such a stack keeps its names)
+        self.norms = torch.nn.ModuleList(N.LayerNorm(d) for d in dims[1:-1]) if norm is not None else None
 
-    def forward(self, features, inputInfo, edge_index=None):
+    def _between(self, h, i, bias, drop):
+        """what stands between layer i and the next: norm, activation, dropout (`drop`: its keywords, or None)"""
+        relu = self.activation is F.relu
+        fused = drop if relu and drop is not None else {}
+        if self.norms is not None:
+            m = self.norms[i]
+            h = N.layer_norm(h, m.weight, m.bias, m.eps, relu=relu, **fused)
+        elif relu:
+            h = N.dropout(h, bias=bias, relu=True, **fused)
+        if not relu:
+            h = self.activation(h)
+            if drop is not None:
+                h = N.dropout(h, **drop)
+        return h
+
+    def forward(self, features, inputInfo, edge_index=None, seed=None, step=0, row_offset=0):
         h = features
+        last = len(self.layers) - 1
         if not torch.is_grad_enabled() and self.activation is F.relu:
-            # inference: bias and ReLU are fused into the store of the gather kernel
+            # inference: bias and ReLU are fused into the store of the gather kernel (with a norm, the ReLU follows that)
             for i, layer in enumerate(self.layers):
-                h = layer.forward_fused(h, inputInfo, relu=i + 1 < len(self.layers))
+                h = layer.forward_fused(h, inputInfo, relu=i < last and self.norms is None)
+                if i < last and self.norms is not None:
+                    h = self._between(h, i, None, None)
             return h
+        counter = self.dropout_source == "counter"
+        if counter and seed is None and self.training and self.dropout > 0:
+            seed = N.draw_seed()
         for i, layer in enumerate(self.layers):
-            if i:
+            if i and not counter:
                 h = F.dropout(h, self.dropout, self.training)
-            h = layer(h, inputInfo)
-            if i + 1 < len(self.layers):
+            # the fused pass adds the bias itself
+            bare = i < last and counter and self.norms is None and self.activation is F.relu
+            h = layer.convolve(h, inputInfo) if bare else layer(h, inputInfo)
+            if i == last:
+                break
+            if counter:
+                drop = dict(p=self.dropout, seed=seed, step=step + (i << 40), row_offset=row_offset, training=self.training)
+                h = self._between(h, i, layer.bias if bare else None, drop)
+            elif self.norms is not None:
+                h = self._between(h, i, None, None)
+            else:
                 h = self.activation(h)
         return h
 
@@ -127,20 +165,34 @@ class SumAggregate(torch.autograd.Function):
 
 
 class ROF_GIN(torch.nn.Module):
-    """GIN: h' = MLP((1 + eps) h + sum_{n in N(v)} h_n), 2-layer MLP per layer, eps fixed."""
+    """GIN: h' = MLP((1 + eps) h + sum_{n in N(v)} h_n), 2-layer MLP per layer, eps fixed.  norm="layer" puts a
+    layer norm in front of the ReLU between two layers; dropout > 0 a dropout behind it (norm.py, one pass)."""
 
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers=3, eps=0.0):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers=3, eps=0.0, norm=None, dropout=0.0):
         super().__init__()
+        if norm not in (None, "layer"):
+            raise ValueError("ROF_GIN: norm is None or 'layer'")
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
         self.mlps = torch.nn.ModuleList(
             torch.nn.Sequential(torch.nn.Linear(a, n_hidden), torch.nn.ReLU(), torch.nn.Linear(n_hidden, b))
             for a, b in zip(dims[:-1], dims[1:]))
-        self.eps = eps
+        self.eps, self.dropout = eps, dropout
+        self.norms = torch.nn.ModuleList(N.LayerNorm(d) for d in dims[1:-1]) if norm is not None else None
 
-    def forward(self, features, plan: AggregationPlan, plan_t=None):
+    def forward(self, features, plan: AggregationPlan, plan_t=None, seed=None, step=0, row_offset=0):
         h = features
+        if seed is None and self.training and self.dropout > 0:
+            seed = N.draw_seed()
         for i, mlp in enumerate(self.mlps):
             h = mlp(SumAggregate.apply(h, plan, plan_t, None, "sum", 1.0 + self.eps))
-            if i + 1 < len(self.mlps):
+            if i + 1 == len(self.mlps):
+                break
+            drop = dict(p=self.dropout, seed=seed, step=step + (i << 40), row_offset=row_offset, training=self.training)
+            if self.norms is not None:
+                m = self.norms[i]
+                h = N.layer_norm(h, m.weight, m.bias, m.eps, relu=True, **drop)
+            elif self.dropout > 0:
+                h = N.dropout(h, relu=True, **drop)
+            else:
                 h = F.relu(h)
         return h

@@ -1,0 +1,265 @@
+"""The operators between two graph layers: layer norm, dropout, and the two in one pass with the ReLU between
+them (include/rof_b200.h: rof_layer_norm_*, rof_dropout_*), with their gradients.
+
+Dropout draws from a counter-based generator: whether element e = (row_offset + row) * width + column of a matrix
+stays is a function of (seed, step, e) and nothing else.  So no mask is stored (the backward pass computes it again),
+a rank that holds a block of rows drops what a single GPU holding all rows would (`row_offset`), and a run is
+repeated by its seed.  `seed` is a number; without one it is drawn from torch's default CPU generator, which
+torch.manual_seed and torch.utils.checkpoint control.  `step` is a number or a one-element int64 CUDA tensor that
+is read when the kernel runs: a captured graph that adds to it draws anew on every replay.  The backward pass
+reads the tensor too: change it after the backward pass only (in eager mode autograd refuses a change in between).
+
+All sums and statistics are held in 32 bits whatever the matrix's type (float32, bfloat16, float16); results
+are rounded once and are the same bit for bit on every call.  As everywhere in this package there is no CPU path.
+"""
+import ctypes
+
+import torch
+
+from . import _native
+from .plan import _device_guard
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_matrix(x, name):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if x.dtype not in DTYPES:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1:
+        raise RuntimeError(f"{name} must have at least one dimension")
+
+
+def _check_vector(v, name, x):
+    if v is None:
+        return
+    if not isinstance(v, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if v.device != x.device or v.dim() != 1 or v.size(0) != x.size(-1):
+        raise RuntimeError(f"{name} must be a vector of {x.size(-1)} entries on x's device, got {tuple(v.shape)} on {v.device}")
+    if v.dtype not in (torch.float32, x.dtype):
+        raise RuntimeError(f"{name} must be float32 or of x's type, got {v.dtype}")
+
+
+def draw_seed():
+    """a seed from torch's default CPU generator; not under capture, where every replay would use the one drawn now"""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a captured dropout needs a seed: one drawn now would be the same on every replay "
+                           "(give `seed`, and a `step` tensor that the graph adds to)")
+    return int(torch.empty((), dtype=torch.int64).random_())
+
+
+def _check_drop(p, seed, step, row_offset, training, x):
+    """-> None (nothing is dropped) or (p, seed, step, step tensor or None, row_offset)"""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if not training or p == 0.0:
+        return None
+    tensor = None
+    if isinstance(step, torch.Tensor):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.device != x.device:
+            raise RuntimeError("step must be a number or a one-element int64 tensor on x's device")
+        step, tensor = 0, step
+    if seed is None:
+        seed = draw_seed()
+    for name, v, top in (("seed", seed, 2 ** 64), ("step", step, 2 ** 64), ("row_offset", row_offset, 2 ** 60)):
+        if not 0 <= v < top:
+            raise ValueError(f"{name} must be in [0, 2**{top.bit_length() - 1}), got {v}")
+    return float(p), int(seed), int(step), tensor, int(row_offset)
+
+
+def _rows(x):
+    """x as [rows, width] with unit column stride: a view where its layout allows it, else a copy"""
+    v = x if x.dim() == 2 else x.unsqueeze(0) if x.dim() == 1 else x.flatten(0, -2)
+    if (v.stride(1) == 1 or v.size(1) <= 1) and (v.stride(0) >= v.size(1) or v.size(0) <= 1):
+        return v
+    return v.contiguous()
+
+
+def _ld(x):
+    return x.stride(0) if x.size(0) > 1 else x.size(1)
+
+
+def _drop_arg(drop):
+    if drop is None:
+        return None
+    p, seed, step, tensor, row_offset = drop
+    return _native.Dropout(p, seed, step, tensor.data_ptr() if tensor is not None else None, row_offset)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _vectors(weight, bias, x):
+    """contiguous vectors of one type -> (weight, bias, type code)"""
+    kinds = {v.dtype for v in (weight, bias) if v is not None}
+    kind = kinds.pop() if len(kinds) == 1 else torch.float32
+    weight, bias = (v if v is None else v.to(kind).contiguous() for v in (weight, bias))
+    return weight, bias, DTYPES[kind]
+
+
+def _workspace(rows, width, device):
+    # torch's caching allocator returns 512-byte aligned blocks
+    return torch.empty(int(_native.cuda().rof_layer_norm_workspace_bytes(rows, width)), dtype=torch.uint8, device=device)
+
+
+def _norm_forward(x, weight, bias, eps, relu, drop, want_stats):
+    v = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((v.size(0), 2), dtype=torch.float32, device=x.device) if want_stats else None
+    weight, bias, kind = _vectors(weight, bias, x)
+    with _device_guard(x.device):
+        _native.check(_native.cuda().rof_layer_norm_forward(
+            DTYPES[x.dtype], v.data_ptr(), _ld(v), v.size(0), v.size(1), kind, _ptr(weight), _ptr(bias), eps, int(relu),
+            _drop_arg(drop), y.data_ptr(), v.size(1), _ptr(stats), _stream(x.device)))
+    return v, y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, relu, drop, step):
+        v, y, stats = _norm_forward(x, weight, bias, eps, relu, drop, True)
+        ctx.save_for_backward(v, weight, bias, stats, step)
+        ctx.relu, ctx.drop, ctx.shape = relu, drop[:3] + drop[4:] if drop else None, x.shape
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        v, weight, bias, stats, step = ctx.saved_tensors
+        drop = ctx.drop[:3] + (step,) + ctx.drop[3:] if ctx.drop else None
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        rows, width = v.shape
+        dy = _rows(grad)
+        dx = torch.empty(ctx.shape, dtype=v.dtype, device=v.device) if need_x else None
+        w, b, kind = _vectors(weight, bias, v)
+        like = w if w is not None else b
+        dw = torch.empty_like(like) if need_w else None
+        db = torch.empty_like(like) if need_b else None
+        ws = _workspace(rows, width, v.device) if need_w or need_b else None
+        with _device_guard(v.device):
+            _native.check(_native.cuda().rof_layer_norm_backward(
+                DTYPES[v.dtype], dy.data_ptr(), _ld(dy), v.data_ptr(), _ld(v), rows, width, kind, _ptr(w), _ptr(b),
+                stats.data_ptr(), int(ctx.relu), _drop_arg(drop), _ptr(dx), width, _ptr(dw), _ptr(db), _ptr(ws),
+                ws.numel() if ws is not None else 0, _stream(v.device)))
+        return (dx, dw.to(weight.dtype) if need_w else None,
+                db.to(bias.dtype) if need_b else None, None, None, None, None)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None, step=0, row_offset=0, training=True):
+    """dropout(relu?(layer norm of x over its last dimension)) in one pass, and one back.
+
+    x: a CUDA tensor [..., width] of float32, bfloat16 or float16 with any strides; weight, bias: vectors of `width`
+    entries, float32 or of x's type, or None; eps >= 0.  relu: apply the ReLU.  p, seed, step, row_offset: the
+    dropout behind it (see `dropout`), only where `training`.  Returns a contiguous tensor like x; gradients flow to x, weight
+    and bias (once: a second derivative is not offered)."""
+    _check_matrix(x, "x")
+    _check_vector(weight, "weight", x)
+    _check_vector(bias, "bias", x)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    drop = _check_drop(p, seed, step, row_offset, training, x)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, float(eps), bool(relu), drop, drop[3] if drop else None)
+    return _norm_forward(x, weight, bias, float(eps), bool(relu), drop, False)[1]
+
+
+def _dropout_forward(x, bias, relu, drop):
+    v = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _, bias, kind = _vectors(None, bias, x)
+    with _device_guard(x.device):
+        _native.check(_native.cuda().rof_dropout_forward(
+            DTYPES[x.dtype], v.data_ptr(), _ld(v), v.size(0), v.size(1), kind, _ptr(bias), int(relu), _drop_arg(drop),
+            y.data_ptr(), v.size(1), _stream(x.device)))
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, relu, drop, step):
+        y = _dropout_forward(x, bias, relu, drop)
+        # behind a ReLU the output says which elements were kept and positive
+        ctx.save_for_backward(y if relu else None, step)
+        ctx.relu, ctx.drop = relu, drop[:3] + drop[4:] if drop else None
+        ctx.bias_kind = bias.dtype if bias is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, step = ctx.saved_tensors
+        drop = ctx.drop[:3] + (step,) + ctx.drop[3:] if ctx.drop else None
+        need_x, need_b = ctx.needs_input_grad[:2]
+        dy = _rows(grad)
+        rows, width = dy.shape
+        dx = torch.empty(grad.shape, dtype=dy.dtype, device=dy.device) if need_x else None
+        db = torch.empty(width, dtype=ctx.bias_kind, device=dy.device) if need_b else None
+        ws = _workspace(rows, width, dy.device) if need_b else None
+        with _device_guard(dy.device):
+            _native.check(_native.cuda().rof_dropout_backward(
+                DTYPES[dy.dtype], dy.data_ptr(), _ld(dy), _ptr(y), width, rows, width,
+                DTYPES[ctx.bias_kind] if need_b else 0, int(ctx.relu), _drop_arg(drop), _ptr(dx), width, _ptr(db), _ptr(ws),
+                ws.numel() if ws is not None else 0, _stream(dy.device)))
+        return dx, db, None, None, None
+
+
+def dropout(x, p=0.0, seed=None, step=0, row_offset=0, training=True, bias=None, relu=False):
+    """dropout(relu?(x + bias)) in one pass, and one back.
+
+    x: a CUDA tensor [..., width] of float32, bfloat16 or float16 with any strides; bias: a vector of `width` entries,
+    float32 or of x's type, or None.  Each element is zeroed with probability p and scaled by 1 / (1 - p) otherwise, only where
+    `training`; p = 1 zeroes everything.  The choice depends on (seed, step, element index) alone, the index counted from
+    row `row_offset` of the whole matrix.  Returns a contiguous tensor like x."""
+    _check_matrix(x, "x")
+    _check_vector(bias, "bias", x)
+    drop = _check_drop(p, seed, step, row_offset, training, x)
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        return _Dropout.apply(x, bias, bool(relu), drop, drop[3] if drop else None)
+    return _dropout_forward(x, bias, bool(relu), drop)
+
+
+class LayerNorm(torch.nn.Module):
+    """layer_norm() with its weight and bias; relu and p: the ReLU and the dropout behind it, in the same pass."""
+
+    def __init__(self, width, eps=1e-5, bias=True, relu=False, p=0.0):
+        super().__init__()
+        self.width, self.eps, self.relu, self.p = width, eps, relu, p
+        self.weight = torch.nn.Parameter(torch.ones(width))
+        if bias:
+            self.bias = torch.nn.Parameter(torch.zeros(width))
+        else:
+            self.register_parameter("bias", None)
+
+    def reset_parameters(self):
+        torch.nn.init.ones_(self.weight)
+        if self.bias is not None:
+            torch.nn.init.zeros_(self.bias)
+
+    def forward(self, x, seed=None, step=0, row_offset=0):
+        return layer_norm(x, self.weight, self.bias, self.eps, self.relu, self.p, seed, step, row_offset, self.training)
+
+    def extra_repr(self):
+        return f"{self.width}, eps={self.eps}, bias={self.bias is not None}, relu={self.relu}, p={self.p}"
+
+
+class Dropout(torch.nn.Module):
+    """dropout() as a module"""
+
+    def __init__(self, p=0.5, relu=False):
+        super().__init__()
+        self.p, self.relu = p, relu
+
+    def forward(self, x, seed=None, step=0, row_offset=0, bias=None):
+        return dropout(x, self.p, seed, step, row_offset, self.training, bias, self.relu)
+
+    def extra_repr(self):
+        return f"p={self.p}, relu={self.relu}"

@@ -141,11 +141,15 @@ class ROF_GCNConv(torch.nn.Module):
         with torch.no_grad():
             self.part_result_cache.zero_()
 
-    def forward(self, x, inputInfo):
+    def convolve(self, x, inputInfo):
+        """A_hat (x W), without the bias"""
         inputInfo.part_result_cache = self.part_result_cache
         inputInfo.dimWorker = self.dimWorker
         inputInfo.transform_order = self.transform_order
-        out = ROF_GCNConvFunc.apply(x, self.weight, inputInfo, self.add_self_loops, self.kernel_type)
+        return ROF_GCNConvFunc.apply(x, self.weight, inputInfo, self.add_self_loops, self.kernel_type)
+
+    def forward(self, x, inputInfo):
+        out = self.convolve(x, inputInfo)
         return out if self.bias is None else out + self.bias
 
     def forward_fused(self, x, inputInfo, relu=False):

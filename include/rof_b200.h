@@ -298,6 +298,70 @@ int rof_shared_open(const unsigned char* handle, void** ptr);
 int rof_shared_close(void* ptr);
 int rof_shared_free(void* ptr);
 
+/*
+ * The operators between two graph layers (no counterpart in upstream, whose model calls torch for its dropout,
+ * ROF_main.py:192-200): layer norm, dropout, and the two in one pass with the ReLU between them.  Matrices are
+ * row-major with `dim` columns and a row stride in elements, of one of the types below (at least aligned to
+ * their elements; rows whose address and stride are multiples of 16 bytes run on 128-bit loads); vectors
+ * (weight, bias and their gradients) are [dim], 32-bit or of the matrix's type (`vdtype`).  Sums, statistics and all arithmetic are
+ * 32-bit; a result is rounded to the matrix's type once.  The calls only enqueue work on `stream`, on the
+ * current device, allocate nothing, and give the same result bit for bit every time.
+ */
+enum rof_dtype { ROF_DTYPE_F32 = 0, ROF_DTYPE_BF16 = 1, ROF_DTYPE_F16 = 2 };
+
+/*
+ * Which elements a dropout keeps.  Element e = (first_row + row) * dim + column is dropped where word e % 4 of
+ * Philox4x32 (seven rounds) at counter (e / 4, step + *step_dev) under the key `seed` is below
+ * p * 2^32 (rounded to a whole number); the others are scaled by 1 / (1 - p).  No mask is stored: the backward
+ * call gets the same rof_dropout and computes the words again, so *step_dev must not change in between.
+ * `first_row` is the matrix's first row in the whole one: ranks that hold row blocks drop
+ * what one GPU holding all rows drops.
+ */
+typedef struct rof_dropout {
+  double p;                 /* in [0, 1]; 1 drops everything */
+  uint64_t seed;
+  uint64_t step;
+  const int64_t* step_dev;  /* device; may be NULL.  Read when the kernel runs: a captured graph that changes it draws anew */
+  int64_t first_row;
+} rof_dropout;
+
+/*
+ * y = drop(relu?((x - mean) * rstd * weight + bias)) for every row, mean and rstd = 1 / sqrt(variance + eps) over its
+ * `dim` columns.  weight (1), bias (0) and drop (nothing dropped) may be NULL.  stats: [rows][2], the rows' mean and rstd for the
+ * backward call; may be NULL.  y must not overlap x.
+ */
+int rof_layer_norm_forward(int dtype, const void* x, int64_t ldx, int64_t rows, int dim, int vdtype, const void* weight,
+                           const void* bias, float eps, int relu, const rof_dropout* drop, void* y, int64_t ldy,
+                           float* stats, void* stream);
+
+/*
+ * Gradients of the call above: dx, dweight = sum over the rows of dz * (x - mean) * rstd, dbias = sum over the rows of dz, where dz
+ * is dy behind the dropout and the ReLU.  Any of the three may be NULL: not computed.  `bias` is read where relu is set.
+ * With no rows dweight and dbias are zeroed.  dx must not overlap x or dy.
+ * workspace: rof_layer_norm_workspace_bytes(rows, dim), 256-byte aligned; needed where dweight or dbias is given.
+ */
+int64_t rof_layer_norm_workspace_bytes(int64_t rows, int dim);
+int rof_layer_norm_backward(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows, int dim,
+                            int vdtype, const void* weight, const void* bias, const float* stats, int relu,
+                            const rof_dropout* drop, void* dx, int64_t lddx, void* dweight, void* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * y = drop(relu?(x + bias)): dropout, with the bias add and the activation that stand before it in a GCN stack
+ * (reuse_conv.py:150, ROF_main.py:181).  bias and drop may be NULL.  y may be x itself.
+ */
+int rof_dropout_forward(int dtype, const void* x, int64_t ldx, int64_t rows, int dim, int vdtype, const void* bias, int relu,
+                        const rof_dropout* drop, void* y, int64_t ldy, void* stream);
+
+/*
+ * Gradients of the call above: dx and dbias = sum over the rows of dx before its rounding; either may be NULL.  With relu, `y` is the forward's
+ * output, which says by itself which elements were kept and positive; without, it is not read and may be NULL.  dx may be dy itself.
+ * workspace as above (rof_layer_norm_workspace_bytes), needed where dbias is given.
+ */
+int rof_dropout_backward(int dtype, const void* dy, int64_t lddy, const void* y, int64_t ldy, int64_t rows, int dim, int vdtype,
+                         int relu, const rof_dropout* drop, void* dx, int64_t lddx, void* dbias, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 /* Reads and clears the plan's device status word: non-zero when a bounded wait inside a kernel
  * of an earlier pass ran out (that pass's output is incomplete).  rof_aggregate() checks it on
  * entry and returns ROF_ERR_WAIT_LIMIT. */
