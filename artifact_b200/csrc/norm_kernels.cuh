@@ -1,0 +1,851 @@
+// Device code of norm.cu, one translation unit per element type (norm_f32.cu, norm_bf16.cu, norm_f16.cu).
+//
+// All of it moves a few bytes per operation and is bound by HBM, so the layout is about keeping 16-byte loads in
+// flight.  A *group* of L threads owns one row at a time and lane i of it the vectors i, i + L, ... of the row (L = 4..32
+// inside a warp, or the whole block for wide rows); weights, biases and the column sums of the backward
+// pass stay in the thread's registers over all its rows.
+//
+// Rows that do not start on a 16-byte boundary (odd widths in contiguous matrices) use the same vectors: vector i of a row
+// starts at column i * VEC - s, where s is the row start's distance from the boundary below it; the first and last
+// vector are then partial and loaded element by element.  s has period VEC in the row number, and the groups advance by a multiple of
+// VEC rows, so a thread's columns never change.  All matrices of a call must share s (EDGE covers it; without
+// EDGE every vector is whole); calls where they do not run on the *_plain kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "norm.h"
+
+namespace rof {
+namespace {
+
+// ---- types --------------------------------------------------------------------------------------
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+template <class T> constexpr int kVec = 16 / (int)sizeof(T);
+
+// a weight or bias vector: 32-bit, or of the matrix's own type
+template <class T>
+__device__ __forceinline__ float vector_at(const void* p, int f32, int i) {
+  return f32 ? __ldg(reinterpret_cast<const float*>(p) + i) : to_float(reinterpret_cast<const T*>(p)[i]);
+}
+
+template <class T>
+__device__ __forceinline__ void vector_put(void* p, int f32, int i, float v) {
+  if (f32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<T*>(p)[i] = from_float<T>(v);
+}
+
+template <class T>
+union Pack {
+  uint4 raw;
+  T v[kVec<T>];
+  __device__ Pack() {}
+};
+
+// columns [c, c + VEC) of a row; what lies outside [0, dim) is zero
+template <class T, bool EDGE>
+__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim) {
+  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
+    out.raw = *reinterpret_cast<const uint4*>(row + c);
+  } else {
+#pragma unroll
+    for (int t = 0; t < kVec<T>; ++t) out.v[t] = (unsigned)(c + t) < (unsigned)dim ? row[c + t] : from_float<T>(0.0f);
+  }
+}
+
+template <class T, bool EDGE>
+__device__ __forceinline__ void store_vec(T* row, int c, int dim, const float (&v)[kVec<T>]) {
+  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
+    Pack<T> p;
+#pragma unroll
+    for (int t = 0; t < kVec<T>; ++t) p.v[t] = from_float<T>(v[t]);
+    *reinterpret_cast<uint4*>(row + c) = p.raw;
+  } else {
+#pragma unroll
+    for (int t = 0; t < kVec<T>; ++t)
+      if ((unsigned)(c + t) < (unsigned)dim) row[c + t] = from_float<T>(v[t]);
+  }
+}
+
+// ---- generator ----------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, uint32_t k0, uint32_t k1) {
+  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)b;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint64_t step_of(const Drop& d) {
+  return d.on && d.step_dev != nullptr ? d.step + (uint64_t)*d.step_dev : d.step;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+__device__ __forceinline__ bool kept(const Drop& d, uint64_t step, int64_t e) {
+  return word(philox7((uint64_t)e >> 2, step, d.k0, d.k1), (int)(e & 3)) > d.last;
+}
+
+// bit t: element e + t stays (N a multiple of 4).  One Philox call gives the words of four elements that start at a multiple of
+// four; elsewhere (EDGE only) the N elements lie in N / 4 + 1 such groups.
+template <int N, bool EDGE>
+__device__ __forceinline__ uint32_t keep_bits(const Drop& d, uint64_t step, int64_t e) {
+  const int sh = EDGE ? (int)(e & 3) : 0;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q) {
+    const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
+    bits |= (uint32_t)(w.x > d.last) << (4 * q);
+    bits |= (uint32_t)(w.y > d.last) << (4 * q + 1);
+    bits |= (uint32_t)(w.z > d.last) << (4 * q + 2);
+    bits |= (uint32_t)(w.w > d.last) << (4 * q + 3);
+  }
+  if (EDGE && sh != 0) {
+    const uint4 w = philox7((uint64_t)(e >> 2) + N / 4, step, d.k0, d.k1);
+    bits |= (uint32_t)(w.x > d.last) << N;
+    bits |= (uint32_t)(w.y > d.last) << (N + 1);
+    bits |= (uint32_t)(w.z > d.last) << (N + 2);
+    bits >>= sh;
+  }
+  return bits;
+}
+
+// relu(z) and its gradient keep a NaN, as torch's do
+__device__ __forceinline__ float relu_of(float z) { return z <= 0.0f ? 0.0f : z; }
+
+__device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
+
+// ---- groups -------------------------------------------------------------------------------------
+// L = 4..32: lanes of a warp; L = 0: the block is the group
+template <int L>
+struct Group {
+  int lane, lanes, index;      // index: of the group in the block
+  unsigned mask;
+  int64_t first, stride;       // rows of this group: first, first + stride, ...
+  __device__ __forceinline__ Group() {
+    if constexpr (L == 0) {
+      lane = threadIdx.x;
+      lanes = blockDim.x;
+      index = 0;
+      mask = 0xffffffffu;
+      first = blockIdx.x;
+      stride = gridDim.x;
+    } else {
+      lane = threadIdx.x % L;
+      lanes = L;
+      index = threadIdx.x / L;
+      mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << ((threadIdx.x & 31) & ~(L - 1));
+      first = (int64_t)blockIdx.x * (blockDim.x / L) + index;
+      stride = (int64_t)gridDim.x * (blockDim.x / L);
+    }
+  }
+  // sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
+  // for each of two sums that follow one another (L = 0 only)
+  __device__ __forceinline__ float2 sum(float2 v, float2* buf) const {
+#pragma unroll
+    for (int o = (L == 0 ? 32 : L) / 2; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(mask, v.x, o);
+      v.y += __shfl_xor_sync(mask, v.y, o);
+    }
+    if constexpr (L == 0) {
+      if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = buf[0];
+      for (int i = 1; i < (int)(blockDim.x >> 5); ++i) {
+        v.x += buf[i].x;
+        v.y += buf[i].y;
+      }
+    }
+    return v;
+  }
+  __device__ __forceinline__ float sum(float v, float2* buf) const {
+    if constexpr (L == 0) {
+      return sum(make_float2(v, 0.0f), buf).x;
+    } else {
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+      return v;
+    }
+  }
+};
+
+// distance of row r's first element from the 16-byte boundary below it
+template <class T, bool EDGE>
+__device__ __forceinline__ int row_shift(const void* base, int64_t ld, int64_t r) {
+  if constexpr (!EDGE) return 0;
+  return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(r * ld)) % kVec<T>);
+}
+
+// ---- layer norm ---------------------------------------------------------------------------------
+template <class T, int L, int C, bool DROP, bool EDGE>
+__global__ void __launch_bounds__(L == 0 ? 512 : 256) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int V = kVec<T>;
+  __shared__ float2 buf[2][32];
+  const Group<L> g;
+  const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  const float inv = 1.0f / (float)a.dim;
+  float w[C][V], b[C][V];
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+#pragma unroll
+    for (int t = 0; t < V; ++t) {
+      const int c = (g.lane + k * g.lanes) * V - s + t;
+      const bool in = (unsigned)c < (unsigned)a.dim;
+      w[k][t] = in && a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
+      b[k][t] = in && a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f;
+    }
+  for (int64_t r = g.first; r < a.rows; r += g.stride) {
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
+    Pack<T> raw[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+      if (c < a.dim) load_vec<T, EDGE>(raw[k], x, c, a.dim);
+      else raw[k].raw = make_uint4(0, 0, 0, 0);
+    }
+    float v[C][V], total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int t = 0; t < V; ++t) {
+        v[k][t] = to_float(raw[k].v[t]);
+        total += v[k][t];
+      }
+    // the mean, corrected by the sum of the deviations from its first value
+    float mean = g.sum(total, buf[0]) * inv;
+    float2 dev = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+#pragma unroll
+      for (int t = 0; t < V; ++t) {
+        const float d = (EDGE ? (unsigned)(c + t) < (unsigned)a.dim : c < a.dim) ? v[k][t] - mean : 0.0f;
+        dev.x += d;
+        dev.y = __fmaf_rn(d, d, dev.y);
+      }
+    }
+    dev = g.sum(dev, buf[1]);
+    const float off = dev.x * inv;
+    mean += off;
+    const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+      if (c >= a.dim) continue;
+      uint32_t keep = 0xffffffffu;
+      if constexpr (DROP) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
+      float o[V];
+#pragma unroll
+      for (int t = 0; t < V; ++t) {
+        float z = affine((v[k][t] - mean) * rstd, w[k][t], b[k][t]);
+        if (a.relu) z = relu_of(z);
+        if constexpr (DROP) z = (keep >> t) & 1 ? z * a.drop.scale : 0.0f;
+        o[t] = z;
+      }
+      store_vec<T, EDGE>(y, c, a.dim, o);
+    }
+  }
+}
+
+// Sums the groups' column sums of a block in order and stores them: out[c] for c in [0, dim).  Group i holds its
+// vectors' elements in `acc`; its columns are shifted by shift(i).
+template <class T, int L, int C, bool EDGE>
+__device__ __forceinline__ void store_columns(const float (&acc)[C][kVec<T>], const Group<L>& g, float* out, int dim,
+                                              const void* base, int64_t ld, float* smem) {
+  constexpr int V = kVec<T>;
+  if constexpr (L == 0) {
+    const int s = row_shift<T, EDGE>(base, ld, g.first);
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int t = 0; t < V; ++t) {
+        const int c = (g.lane + k * g.lanes) * V - s + t;
+        if ((unsigned)c < (unsigned)dim) out[c] = acc[k][t];
+      }
+  } else {
+    constexpr int kWidth = L * C * V, kGroups = 256 / L;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int t = 0; t < V; ++t) smem[g.index * kWidth + (g.lane + k * L) * V + t] = acc[k][t];
+    __syncthreads();
+    for (int c = threadIdx.x; c < dim; c += 256) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        sum += smem[i * kWidth + c + row_shift<T, EDGE>(base, ld, (int64_t)blockIdx.x * kGroups + i)];
+      out[c] = sum;
+    }
+  }
+}
+
+// dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
+template <class T, int L, int C, bool DROP, bool EDGE>
+__global__ void __launch_bounds__(L == 0 ? 512 : 256) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int V = kVec<T>;
+  __shared__ float2 buf[2][32];
+  extern __shared__ float columns[];
+  const Group<L> g;
+  const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  const float inv = 1.0f / (float)a.dim;
+  float w[C][V], b[C][V], aw[C][V], ab[C][V];
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+#pragma unroll
+    for (int t = 0; t < V; ++t) {
+      const int c = (g.lane + k * g.lanes) * V - s + t;
+      const bool in = (unsigned)c < (unsigned)a.dim;
+      w[k][t] = in && a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
+      b[k][t] = in && a.relu && a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f;
+      aw[k][t] = ab[k][t] = 0.0f;
+    }
+  int turn = 0;
+  for (int64_t r = g.first; r < a.rows; r += g.stride, turn ^= 1) {
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + r * a.lddy;
+    Pack<T> rx[C], rd[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+      if (c < a.dim) {
+        load_vec<T, EDGE>(rx[k], x, c, a.dim);
+        load_vec<T, EDGE>(rd[k], dy, c, a.dim);
+      } else {
+        rx[k].raw = rd[k].raw = make_uint4(0, 0, 0, 0);
+      }
+    }
+    const float2 st = a.stats[r];
+    float h[C][V], gr[C][V];
+    float2 sums = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+      uint32_t keep = 0xffffffffu;
+      if constexpr (DROP) {
+        if (c < a.dim) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
+      }
+#pragma unroll
+      for (int t = 0; t < V; ++t) {
+        // a column outside the row has dy = 0 and adds nothing anywhere
+        const bool in = EDGE ? (unsigned)(c + t) < (unsigned)a.dim : c < a.dim;
+        h[k][t] = in ? (to_float(rx[k].v[t]) - st.x) * st.y : 0.0f;
+        float dz = to_float(rd[k].v[t]);
+        if constexpr (DROP) dz = (keep >> t) & 1 ? dz * a.drop.scale : 0.0f;
+        if (a.relu && affine(h[k][t], w[k][t], b[k][t]) <= 0.0f) dz = 0.0f;
+        aw[k][t] = __fmaf_rn(dz, h[k][t], aw[k][t]);
+        ab[k][t] += dz;
+        gr[k][t] = dz * w[k][t];
+        sums.x += gr[k][t];
+        sums.y = __fmaf_rn(gr[k][t], h[k][t], sums.y);
+      }
+    }
+    if (a.out == nullptr) continue;
+    T* dx = reinterpret_cast<T*>(a.out) + r * a.ldo;
+    sums = g.sum(sums, buf[turn]);
+    const float c1 = sums.x * inv, c2 = sums.y * inv;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = (g.lane + k * g.lanes) * V - s;
+      if (c >= a.dim) continue;
+      float o[V];
+#pragma unroll
+      for (int t = 0; t < V; ++t) o[t] = st.y * (gr[k][t] - __fmaf_rn(h[k][t], c2, c1));
+      store_vec<T, EDGE>(dx, c, a.dim, o);
+    }
+  }
+  if (a.partial != nullptr) {
+    float* p = a.partial + (int64_t)blockIdx.x * 2 * a.dim;
+    store_columns<T, L, C, EDGE>(aw, g, p, a.dim, a.x, a.ldx, columns);
+    store_columns<T, L, C, EDGE>(ab, g, p + a.dim, a.dim, a.x, a.ldx, columns);
+  }
+}
+
+// out[i] = sum over the blocks' partial[block][i] for i in [0, width): eight runs of blocks per column, added in order.  Columns
+// up to `split` go to `first`, the others to `second`.
+template <class T>
+__global__ void __launch_bounds__(256) join_columns_kernel(const float* partial, int blocks, int width, int split, void* first, void* second, int f32) {
+  __shared__ float part[8][33];
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, i = blockIdx.x * 32 + x;
+  float sum = 0.0f;
+  if (i < width) {
+#pragma unroll 8
+    for (int k = run; k < blocks; k += 8) sum += partial[(int64_t)k * width + i];
+  }
+  part[run][x] = sum;
+  __syncthreads();
+  if (run == 0 && i < width) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) sum += part[k][x];
+    void* out = i < split ? first : second;
+    if (out != nullptr) vector_put<T>(out, f32, i < split ? i : i - split, sum);
+  }
+}
+
+// ---- layer norm, any alignment and width ---------------------------------------------------------
+// One block per row and one element per load, for matrices whose rows lie differently against the 16-byte boundaries and for rows
+// wider than a block's registers; the row is read again instead of kept.
+template <class T>
+__global__ void __launch_bounds__(256) norm_forward_plain(const __grid_constant__ NormArgs a) {
+  __shared__ float2 buf[2][32];
+  const Group<0> g;
+  const uint64_t step = step_of(a.drop);
+  const float inv = 1.0f / (float)a.dim;
+  for (int64_t r = g.first; r < a.rows; r += g.stride) {
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
+    float total = 0.0f;
+    for (int c = g.lane; c < a.dim; c += g.lanes) total += to_float(x[c]);
+    float mean = g.sum(total, buf[0]) * inv;
+    float2 dev = make_float2(0.0f, 0.0f);
+    for (int c = g.lane; c < a.dim; c += g.lanes) {
+      const float d = to_float(x[c]) - mean;
+      dev.x += d;
+      dev.y = __fmaf_rn(d, d, dev.y);
+    }
+    dev = g.sum(dev, buf[1]);
+    const float off = dev.x * inv;
+    mean += off;
+    const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+    for (int c = g.lane; c < a.dim; c += g.lanes) {
+      float z = affine((to_float(x[c]) - mean) * rstd, a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f,
+                       a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f);
+      if (a.relu) z = relu_of(z);
+      if (a.drop.on) z = kept(a.drop, step, a.drop.first + r * a.dim + c) ? z * a.drop.scale : 0.0f;
+      y[c] = from_float<T>(z);
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ float norm_dz(const NormArgs& a, uint64_t step, int64_t r, int c, float h, float w) {
+  float dz = to_float(reinterpret_cast<const T*>(a.dy)[r * a.lddy + c]);
+  if (a.drop.on) dz = kept(a.drop, step, a.drop.first + r * a.dim + c) ? dz * a.drop.scale : 0.0f;
+  if (a.relu && affine(h, w, a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f) <= 0.0f) dz = 0.0f;
+  return dz;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) norm_backward_rows_plain(const __grid_constant__ NormArgs a) {
+  __shared__ float2 buf[2][32];
+  const Group<0> g;
+  const uint64_t step = step_of(a.drop);
+  const float inv = 1.0f / (float)a.dim;
+  int turn = 0;
+  for (int64_t r = g.first; r < a.rows; r += g.stride, turn ^= 1) {
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    T* dx = reinterpret_cast<T*>(a.out) + r * a.ldo;
+    const float2 st = a.stats[r];
+    float2 sums = make_float2(0.0f, 0.0f);
+    for (int c = g.lane; c < a.dim; c += g.lanes) {
+      const float h = (to_float(x[c]) - st.x) * st.y, w = a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
+      const float gr = w * norm_dz<T>(a, step, r, c, h, w);
+      sums.x += gr;
+      sums.y = __fmaf_rn(gr, h, sums.y);
+    }
+    sums = g.sum(sums, buf[turn]);
+    const float c1 = sums.x * inv, c2 = sums.y * inv;
+    for (int c = g.lane; c < a.dim; c += g.lanes) {
+      const float h = (to_float(x[c]) - st.x) * st.y, w = a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
+      dx[c] = from_float<T>(st.y * (w * norm_dz<T>(a, step, r, c, h, w) - __fmaf_rn(h, c2, c1)));
+    }
+  }
+}
+
+// thread = column, blockIdx.y = a run of rows
+template <class T>
+__global__ void __launch_bounds__(128) norm_backward_columns_plain(const __grid_constant__ NormArgs a, int64_t run_rows) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= a.dim) return;
+  const uint64_t step = step_of(a.drop);
+  const float w = a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
+  const int64_t r0 = (int64_t)blockIdx.y * run_rows, r1 = min(a.rows, r0 + run_rows);
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const float2 st = a.stats[r];
+    const float h = (to_float(reinterpret_cast<const T*>(a.x)[r * a.ldx + c]) - st.x) * st.y;
+    const float dz = norm_dz<T>(a, step, r, c, h, w);
+    s1 = __fmaf_rn(dz, h, s1);
+    s2 += dz;
+  }
+  a.partial[((int64_t)blockIdx.y * 2 + 0) * a.dim + c] = s1;
+  a.partial[((int64_t)blockIdx.y * 2 + 1) * a.dim + c] = s2;
+}
+
+// ---- dropout ------------------------------------------------------------------------------------
+// one vector: BACK = false: drop(relu?(x + b)); BACK = true: dy behind the dropout and the ReLU, where with the ReLU
+// the forward's output y says which elements were kept and positive
+template <class T, bool BACK, bool EDGE>
+__device__ __forceinline__ void drop_vec(const DropArgs& a, uint64_t step, int64_t e, const Pack<T>& in, const Pack<T>& y,
+                                         const float (&b)[kVec<T>], float (&o)[kVec<T>]) {
+  constexpr int V = kVec<T>;
+  const bool draw = a.drop.on && !(BACK && a.relu);
+  const uint32_t keep = draw ? keep_bits<V, EDGE>(a.drop, step, e) : 0xffffffffu;
+#pragma unroll
+  for (int t = 0; t < V; ++t) {
+    float z = to_float(in.v[t]);
+    if constexpr (BACK) {
+      z = ((keep >> t) & 1) && !(a.relu && to_float(y.v[t]) <= 0.0f) ? z * a.drop.scale : 0.0f;
+    } else {
+      z += b[t];
+      if (a.relu) z = relu_of(z);
+      z = (keep >> t) & 1 ? z * a.drop.scale : 0.0f;
+    }
+    o[t] = z;
+  }
+}
+
+// contiguous matrices without a bias: one run of n elements from an aligned address
+template <class T, bool BACK, bool EDGE>
+__global__ void __launch_bounds__(256) dropout_flat_kernel(const __grid_constant__ DropArgs a, int64_t n) {
+  constexpr int V = kVec<T>, U = 2;
+  const uint64_t step = step_of(a.drop);
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* y = reinterpret_cast<const T*>(a.y);
+  T* out = reinterpret_cast<T*>(a.out);
+  const bool two = BACK && a.relu;
+  const float zero[V] = {};
+  const int64_t vectors = n / V, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vectors; i += U * stride) {
+    Pack<T> in[U], yy[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * stride < vectors) {
+        in[u].raw = reinterpret_cast<const uint4*>(x)[i + u * stride];
+        if (two) yy[u].raw = reinterpret_cast<const uint4*>(y)[i + u * stride];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * stride < vectors) {
+        float o[V];
+        const int64_t e = (i + u * stride) * V;
+        drop_vec<T, BACK, EDGE>(a, step, a.drop.first + e, in[u], yy[u], zero, o);
+        Pack<T> p;
+#pragma unroll
+        for (int t = 0; t < V; ++t) p.v[t] = from_float<T>(o[t]);
+        reinterpret_cast<uint4*>(out)[i + u * stride] = p.raw;
+      }
+  }
+  // the last elements that fill no vector
+  const int64_t e = vectors * V + threadIdx.x;
+  if (blockIdx.x == 0 && e < n) {
+    float z = to_float(x[e]);
+    const bool keep = !a.drop.on || two || kept(a.drop, step, a.drop.first + e);
+    if (!BACK && a.relu) z = relu_of(z);
+    if (two && to_float(y[e]) <= 0.0f) z = 0.0f;
+    out[e] = from_float<T>(keep ? z * a.drop.scale : 0.0f);
+  }
+}
+
+// thread = vector `col` of the rows row0, row0 + stride, ...; a.lanes threads side by side cover a tile of a row
+template <class T, bool BACK, bool EDGE>
+__global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
+  constexpr int V = kVec<T>, U = 4;
+  extern __shared__ float columns[];
+  const int groups = blockDim.x / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes;
+  const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
+  const int s = row_shift<T, EDGE>(a.x, a.ldx, first);
+  const int c = (int)(blockIdx.y * a.lanes + lane) * V - s;
+  const bool live = group < groups && c < a.dim;
+  const uint64_t step = step_of(a.drop);
+  const bool two = BACK && a.relu;
+  float b[V], acc[V];
+#pragma unroll
+  for (int t = 0; t < V; ++t) {
+    b[t] = !BACK && live && a.bias != nullptr && (unsigned)(c + t) < (unsigned)a.dim ? vector_at<T>(a.bias, a.bf32, c + t) : 0.0f;
+    acc[t] = 0.0f;
+  }
+  if (live) {
+    for (int64_t r = first; r < a.rows; r += U * stride) {
+      Pack<T> in[U], yy[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * stride < a.rows) {
+          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim);
+          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * stride < a.rows) {
+          float o[V];
+          drop_vec<T, BACK, EDGE>(a, step, a.drop.first + (r + u * stride) * a.dim + c, in[u], yy[u], b, o);
+          if constexpr (BACK) {
+#pragma unroll
+            for (int t = 0; t < V; ++t) acc[t] += o[t];
+          }
+          if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o);
+        }
+    }
+  }
+  if (!BACK || a.partial == nullptr) return;
+  if (group < groups) {
+#pragma unroll
+    for (int t = 0; t < V; ++t) columns[(group * a.lanes + lane) * V + t] = live ? acc[t] : 0.0f;
+  }
+  __syncthreads();
+  const int tile = a.lanes * V, c0 = blockIdx.y * tile;
+  // Group k holds columns [c0 - shift, c0 - shift + tile).  With more than one tile a block has one group, so the tiles' columns
+  // neither overlap nor leave a gap.
+  float* p = a.partial + (int64_t)blockIdx.x * a.dim;
+  for (int i = threadIdx.x; i < tile + (EDGE ? V : 0); i += blockDim.x) {
+    float sum = 0.0f;
+    const int col = c0 - (EDGE ? V : 0) + i;
+    bool any = false;
+    for (int k = 0; k < groups; ++k) {
+      const int j = col - c0 + row_shift<T, EDGE>(a.x, a.ldx, (int64_t)blockIdx.x * groups + k);
+      if (j >= 0 && j < tile) {
+        sum += columns[k * tile + j];
+        any = true;
+      }
+    }
+    if (any && (unsigned)col < (unsigned)a.dim) p[col] = sum;
+  }
+}
+
+template <class T, bool BACK>
+__global__ void __launch_bounds__(256) dropout_plain(const __grid_constant__ DropArgs a) {
+  const uint64_t step = step_of(a.drop);
+  const int64_t n = a.rows * a.dim, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const int64_t r = i / a.dim;
+    const int c = (int)(i - r * a.dim);
+    float z = to_float(reinterpret_cast<const T*>(a.x)[r * a.ldx + c]);
+    const bool two = BACK && a.relu;
+    bool keep = !a.drop.on || two || kept(a.drop, step, a.drop.first + i);
+    if constexpr (BACK) {
+      keep = keep && !(two && to_float(reinterpret_cast<const T*>(a.y)[r * a.ldy + c]) <= 0.0f);
+    } else {
+      if (a.bias != nullptr) z += vector_at<T>(a.bias, a.bf32, c);
+      if (a.relu) z = relu_of(z);
+    }
+    reinterpret_cast<T*>(a.out)[r * a.ldo + c] = from_float<T>(keep ? z * a.drop.scale : 0.0f);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(128) dropout_columns_plain(const __grid_constant__ DropArgs a, int64_t run_rows) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= a.dim) return;
+  const uint64_t step = step_of(a.drop);
+  const int64_t r0 = (int64_t)blockIdx.y * run_rows, r1 = min(a.rows, r0 + run_rows);
+  float sum = 0.0f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const bool keep = a.relu ? !(to_float(reinterpret_cast<const T*>(a.y)[r * a.ldy + c]) <= 0.0f)
+                             : !a.drop.on || kept(a.drop, step, a.drop.first + r * a.dim + c);
+    if (keep) sum += to_float(reinterpret_cast<const T*>(a.x)[r * a.ldx + c]) * a.drop.scale;
+  }
+  a.partial[(int64_t)blockIdx.y * a.dim + c] = sum;
+}
+
+// ---- launches -----------------------------------------------------------------------------------
+constexpr int kSMs = 148;
+
+// How the rows of a call's matrices lie against the 16-byte boundaries.  vec: the same way in all of them; edge: there are
+// partial vectors; vectors: of a row, at most.
+struct Layout {
+  bool vec, edge;
+  int vectors;
+};
+
+struct Matrix {
+  const void* p;
+  int64_t ld;
+};
+
+template <class T>
+Layout layout_of(int64_t rows, int dim, std::initializer_list<Matrix> all) {
+  constexpr int V = kVec<T>;
+  int start = -1, advance = -1;
+  for (const Matrix& m : all) {
+    if (m.p == nullptr) continue;
+    const int s = (int)(reinterpret_cast<uintptr_t>(m.p) / sizeof(T) % V), d = rows > 1 ? (int)(m.ld % V) : 0;
+    if (start >= 0 && (s != start || d != advance)) return {false, true, 0};
+    start = s;
+    advance = d;
+  }
+  if (start < 0) start = advance = 0;             // no rows
+  int gcd = V;                                    // the rows' starts are congruent modulo this
+  while (advance % gcd) gcd /= 2;
+  const int most = V - gcd + start % gcd;
+  const int shift = advance == 0 ? start : most;
+  return {true, dim % V != 0 || shift != 0, (int)(((int64_t)dim + shift + V - 1) / V)};
+}
+
+template <class K>
+int blocks_per_sm(K kernel, int threads, int smem) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
+}
+
+inline int clamp_blocks(int64_t wanted, int64_t most) { return (int)std::max<int64_t>(1, std::min(wanted, most)); }
+
+// group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads)
+template <class T, class F>
+bool by_width(int vectors, F&& f) {
+  constexpr bool wide = sizeof(T) == 4;          // 16 (20) elements per thread either way
+  if (vectors <= 4) f.template operator()<4, 1>(256);
+  else if (vectors <= 8) f.template operator()<8, 1>(256);
+  else if (vectors <= 16) f.template operator()<16, 1>(256);
+  else if (vectors <= 32) f.template operator()<32, 1>(256);
+  else if (vectors <= 64) f.template operator()<32, 2>(256);
+  else if (wide && vectors <= 96) f.template operator()<32, wide ? 3 : 2>(256);
+  else if (wide && vectors <= 128) f.template operator()<32, wide ? 4 : 2>(256);
+  else if (wide && vectors <= 160) f.template operator()<32, wide ? 5 : 2>(256);
+  else {
+    constexpr int C = wide ? 4 : 2;
+    const int threads = ((vectors + C - 1) / C + 31) / 32 * 32;
+    if (threads > 512) return false;
+    f.template operator()<0, C>(threads);
+  }
+  return true;
+}
+
+template <class T, bool DROP, bool EDGE>
+struct NormForward {
+  const NormArgs& a;
+  cudaStream_t stream;
+  template <int L, int C>
+  void operator()(int threads) const {
+    auto kernel = norm_forward_kernel<T, L, C, DROP, EDGE>;
+    static const int full = blocks_per_sm(kernel, L == 0 ? 256 : 256, 0);
+    constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
+    int64_t most = (int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full);
+    int blocks = clamp_blocks((a.rows + per - 1) / per, most);
+    if (L == 0) blocks = (blocks + 7) / 8 * 8;
+    kernel<<<blocks, threads, 0, stream>>>(a);
+  }
+};
+
+template <class T, bool DROP, bool EDGE>
+struct NormBackward {
+  const NormArgs& a;
+  cudaStream_t stream;
+  int* blocks;
+  template <int L, int C>
+  void operator()(int threads) const {
+    auto kernel = norm_backward_kernel<T, L, C, DROP, EDGE>;
+    constexpr int smem = L == 0 ? 0 : 256 * C * kVec<T> * 4;
+    static const int full = blocks_per_sm(kernel, 256, smem);
+    constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
+    const int64_t most = std::min<int64_t>((int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full), column_blocks_cap(a.rows, a.dim));
+    *blocks = clamp_blocks((a.rows + per - 1) / per, most);
+    if (L == 0) *blocks = *blocks < 8 ? 8 : *blocks / 8 * 8;
+    kernel<<<*blocks, threads, smem, stream>>>(a);
+  }
+};
+
+template <class T>
+cudaError_t launch_join(const float* partial, int blocks, int width, int split, void* first, void* second, int f32, cudaStream_t stream) {
+  join_columns_kernel<T><<<(width + 31) / 32, 256, 0, stream>>>(partial, blocks, width, split, first, second, f32);
+  return cudaGetLastError();
+}
+
+// (a single row has no row stride; the kernels' shifts of rows that do not exist must not depend on one)
+inline NormArgs one_row(NormArgs a) {
+  if (a.rows <= 1) a.ldx = a.lddy = a.ldo = 0;
+  return a;
+}
+
+template <class T>
+cudaError_t launch_norm_forward(const NormArgs& given, cudaStream_t stream) {
+  const NormArgs a = one_row(given);
+  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
+  bool done = false;
+  if (l.vec) {
+    if (a.drop.on) done = l.edge ? by_width<T>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, true, false>{a, stream});
+    else done = l.edge ? by_width<T>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, false, false>{a, stream});
+  }
+  if (!done) norm_forward_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
+  const NormArgs a = one_row(given);
+  int blocks = 0;
+  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
+  bool done = false;
+  if (l.vec) {
+    if (a.drop.on) done = l.edge ? by_width<T>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
+    else done = l.edge ? by_width<T>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
+  }
+  if (!done) {
+    if (a.out != nullptr) norm_backward_rows_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
+    if (a.partial != nullptr) {
+      blocks = clamp_blocks((a.rows + 31) / 32, column_blocks_cap(a.rows, a.dim));
+      norm_backward_columns_plain<T><<<dim3((a.dim + 127) / 128, blocks), 128, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);
+    }
+  }
+  if (a.partial == nullptr) return cudaGetLastError();
+  return launch_join<T>(a.partial, blocks, 2 * a.dim, a.dim, a.dweight, a.dbias, a.wf32, stream);
+}
+
+template <class T, bool BACK>
+cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
+  DropArgs a = given;
+  if (a.rows <= 1) a.ldx = a.ldy = a.ldo = 0;
+  constexpr int V = kVec<T>;
+  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.y, a.ldy}, {a.out, a.ldo}});
+  const auto whole = [&](const void* p, int64_t ld) {
+    return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (a.rows == 1 || ld == a.dim));
+  };
+  if (a.partial == nullptr && a.bias == nullptr && whole(a.x, a.ldx) && whole(a.y, a.ldy) && whole(a.out, a.ldo)) {
+    const int64_t n = a.rows * a.dim;
+    const int blocks = clamp_blocks((n / V + 511) / 512, kSMs * 16);
+    if (a.drop.first % 4 == 0) dropout_flat_kernel<T, BACK, false><<<blocks, 256, 0, stream>>>(a, n);
+    else dropout_flat_kernel<T, BACK, true><<<blocks, 256, 0, stream>>>(a, n);
+    return cudaGetLastError();
+  }
+  const int tiles = (l.vectors + 255) / 256;
+  int blocks = 0;
+  if (l.vec && tiles <= 65535) {
+    a.lanes = std::min(l.vectors, 256);
+    const int groups = 256 / a.lanes, threads = (groups * a.lanes + 31) / 32 * 32;
+    const int64_t most = a.partial != nullptr ? column_blocks_cap(a.rows, a.dim) : kMaxColumnBlocks;
+    blocks = clamp_blocks((a.rows + groups - 1) / groups, std::max<int64_t>(most / tiles, 8));
+    blocks = blocks < 8 ? 8 : blocks / 8 * 8;
+    const int smem = BACK && a.partial != nullptr ? groups * a.lanes * V * 4 : 0;
+    const dim3 grid(blocks, tiles);
+    if (l.edge) dropout_rows_kernel<T, BACK, true><<<grid, threads, smem, stream>>>(a);
+    else dropout_rows_kernel<T, BACK, false><<<grid, threads, smem, stream>>>(a);
+  } else {
+    if (a.out != nullptr) dropout_plain<T, BACK><<<clamp_blocks((a.rows * a.dim + 255) / 256, kSMs * 8), 256, 0, stream>>>(a);
+    if (BACK && a.partial != nullptr) {
+      blocks = clamp_blocks((a.rows + 31) / 32, column_blocks_cap(a.rows, a.dim));
+      dropout_columns_plain<T><<<dim3((a.dim + 127) / 128, blocks), 128, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);
+    }
+  }
+  if (!BACK || a.partial == nullptr) return cudaGetLastError();
+  return launch_join<T>(a.partial, blocks, a.dim, 0, nullptr, a.dbias, a.bf32, stream);
+}
+
+}  // namespace
+
+template <class T>
+constexpr NormLaunchers launchers() {
+  return {launch_norm_forward<T>, launch_norm_backward<T>, launch_dropout<T, false>, launch_dropout<T, true>};
+}
+
+}  // namespace rof
