@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 
 #include "norm.h"
@@ -63,19 +64,61 @@ __device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int 
   }
 }
 
+__device__ __forceinline__ void pack_two(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+__device__ __forceinline__ void pack_two(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void pack_two(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
+
 template <class T, bool EDGE>
-__device__ __forceinline__ void store_vec(T* row, int c, int dim, const float (&v)[kVec<T>]) {
-  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
-    Pack<T> p;
+__device__ __forceinline__ void store_vec(T* row, int c, int dim, const float2 (&v)[kVec<T> / 2]) {
+  Pack<T> p;
 #pragma unroll
-    for (int t = 0; t < kVec<T>; ++t) p.v[t] = from_float<T>(v[t]);
+  for (int t = 0; t < kVec<T> / 2; ++t) pack_two(&p.v[2 * t], v[t]);
+  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
     *reinterpret_cast<uint4*>(row + c) = p.raw;
   } else {
 #pragma unroll
     for (int t = 0; t < kVec<T>; ++t)
-      if ((unsigned)(c + t) < (unsigned)dim) row[c + t] = from_float<T>(v[t]);
+      if ((unsigned)(c + t) < (unsigned)dim) row[c + t] = p.v[t];
   }
 }
+
+// ---- asynchronous copies -------------------------------------------------------------------------
+// 16 bytes from global to shared memory, the last 16 - bytes of them zero and not read
+__device__ __forceinline__ void copy_async(uint4* to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A thread's own ring of S slots in shared memory for the C vectors of its next rows.  Every thread reads only what it copied
+// itself, so the ring needs no barrier: it is an extension of the registers that keeps (S - 1) C vectors a thread in
+// flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.
+template <class T, int C, int S, bool EDGE>
+struct Ring {
+  uint4* mine;
+  int threads;
+  __device__ __forceinline__ Ring(uint4* smem, int part) : mine(smem + (size_t)part * S * C * blockDim.x + threadIdx.x), threads(blockDim.x) {}
+  // columns [c0 + k advance, + VEC) of `row`; what lies behind the row is zero.  In front of it (c0 < 0) the vector holds what
+  // the 16 bytes hold: the end of the row before, or what precedes the matrix in its allocation; zero_front() clears it.
+  __device__ __forceinline__ void fetch(int slot, const T* row, int c0, int advance, int dim) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = c0 + k * advance, left = (dim - c) * (int)sizeof(T);
+      const int bytes = EDGE ? max(0, min(16, left)) : (left > 0 ? 16 : 0);
+      copy_async(mine + (slot * C + k) * threads, row + (bytes > 0 ? c : c0), bytes);
+    }
+  }
+  __device__ __forceinline__ void read(int slot, Pack<T> (&out)[C], int c0) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) out[k].raw = mine[(slot * C + k) * threads];
+    if (EDGE && c0 < 0) {
+#pragma unroll
+      for (int t = 0; t < kVec<T>; ++t)
+        if (c0 + t < 0) out[0].v[t] = from_float<T>(0.0f);
+    }
+  }
+};
 
 // ---- generator ----------------------------------------------------------------------------------
 __device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, uint32_t k0, uint32_t k1) {
@@ -131,6 +174,17 @@ __device__ __forceinline__ uint32_t keep_bits(const Drop& d, uint64_t step, int6
 __device__ __forceinline__ float relu_of(float z) { return z <= 0.0f ? 0.0f : z; }
 
 __device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
+
+// Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+template <class T>
+__device__ __forceinline__ void unpack(const Pack<T>& p, float2 (&v)[kVec<T> / 2]) {
+#pragma unroll
+  for (int t = 0; t < kVec<T> / 2; ++t) v[t] = make_float2(to_float(p.v[2 * t]), to_float(p.v[2 * t + 1]));
+}
+
+__device__ __forceinline__ float half_of(const float2& v, int i) { return i ? v.y : v.x; }
 
 // ---- groups -------------------------------------------------------------------------------------
 // L = 4..32: lanes of a warp; L = 0: the block is the group
@@ -193,74 +247,123 @@ __device__ __forceinline__ int row_shift(const void* base, int64_t ld, int64_t r
   return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(r * ld)) % kVec<T>);
 }
 
+// Blocks of 256 threads per SM that the register allocation aims at: as many as leave nothing spilled.
+template <class T, int C, bool HIDDEN>
+constexpr int forward_blocks() { return C * kVec<T> <= 8 ? 4 : C * kVec<T> <= (HIDDEN ? 12 : 16) ? 3 : 2; }
+template <class T, int C, bool HIDDEN>
+constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? 2 : 1; }
+// Slots of the rings
+template <int C>
+constexpr int ring_slots() { return C == 1 ? 4 : C <= 4 ? 3 : 2; }
+
 // ---- layer norm ---------------------------------------------------------------------------------
-template <class T, int L, int C, bool DROP, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256) norm_forward_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int V = kVec<T>;
-  __shared__ float2 buf[2][32];
-  const Group<L> g;
-  const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
-  const uint64_t step = DROP ? step_of(a.drop) : 0;
-  const float inv = 1.0f / (float)a.dim;
-  float w[C][V], b[C][V];
+// the thread's entries of a vector (`other` where there is none)
+template <class T, int C>
+__device__ __forceinline__ void load_columns(float2 (&out)[C][kVec<T> / 2], const void* p, int f32, int dim, int c0, int advance, float other) {
 #pragma unroll
   for (int k = 0; k < C; ++k)
 #pragma unroll
-    for (int t = 0; t < V; ++t) {
-      const int c = (g.lane + k * g.lanes) * V - s + t;
-      const bool in = (unsigned)c < (unsigned)a.dim;
-      w[k][t] = in && a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
-      b[k][t] = in && a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f;
+    for (int t = 0; t < kVec<T> / 2; ++t) {
+      const int c = c0 + k * advance + 2 * t;
+      out[k][t].x = p != nullptr && (unsigned)c < (unsigned)dim ? vector_at<T>(p, f32, c) : other;
+      out[k][t].y = p != nullptr && (unsigned)(c + 1) < (unsigned)dim ? vector_at<T>(p, f32, c + 1) : other;
     }
+}
+
+// bits 2t and 2t + 1 of `keep` choose between v and zero
+__device__ __forceinline__ float2 select(uint32_t keep, int t, float2 v) {
+  return make_float2((keep >> (2 * t)) & 1 ? v.x : 0.0f, (keep >> (2 * t + 1)) & 1 ? v.y : 0.0f);
+}
+
+// What is computed from v is computed where it is used: the comparisons of a thread's columns with the ends of the row do not
+// change from row to row, but kept over the loop they cost more registers than the row itself.
+__device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v)); }
+
+// HIDDEN: with the ReLU or the dropout (or both)
+template <class T, int L, int C, bool HIDDEN, bool EDGE>
+__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int V = kVec<T>, H = V / 2;
+  __shared__ float2 buf[2][32];
+  extern __shared__ uint4 ring_memory[];
+  const Group<L> g;
+  const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
+  int c0 = g.lane * V - s;
+  const int advance = g.lanes * V;
+  const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
+  const float inv = 1.0f / (float)a.dim;
+  constexpr int S = ring_slots<C>();
+  const Ring<T, C, S, EDGE> ring(ring_memory, 0);
+  const T* x = reinterpret_cast<const T*>(a.x);
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    const int64_t r = g.first + i * g.stride;
+    if (r < a.rows) ring.fetch(i, x + r * a.ldx, c0, advance, a.dim);
+    copy_commit();
+  }
+  float2 w[C][H], b[C][H];
+  load_columns<T, C>(w, a.weight, a.wf32, a.dim, c0, advance, 1.0f);
+  load_columns<T, C>(b, a.bias, a.wf32, a.dim, c0, advance, 0.0f);
+  int slot = 0;
   for (int64_t r = g.first; r < a.rows; r += g.stride) {
-    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
-    T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
+    if constexpr (EDGE) not_hoisted(c0);
     Pack<T> raw[C];
+    copy_wait<S - 2>();
+    ring.read(slot, raw, c0);
+    const int64_t ahead = r + (S - 1) * g.stride;
+    if (ahead < a.rows) ring.fetch(slot == 0 ? S - 1 : slot - 1, x + ahead * a.ldx, c0, advance, a.dim);
+    copy_commit();
+    slot = slot == S - 1 ? 0 : slot + 1;
+    float2 v[C][H], total = both(0.0f);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
-      if (c < a.dim) load_vec<T, EDGE>(raw[k], x, c, a.dim);
-      else raw[k].raw = make_uint4(0, 0, 0, 0);
+      unpack<T>(raw[k], v[k]);
+#pragma unroll
+      for (int t = 0; t < H; ++t) total = __fadd2_rn(total, v[k][t]);
     }
-    float v[C][V], total = 0.0f;
-#pragma unroll
-    for (int k = 0; k < C; ++k)
-#pragma unroll
-      for (int t = 0; t < V; ++t) {
-        v[k][t] = to_float(raw[k].v[t]);
-        total += v[k][t];
-      }
     // the mean, corrected by the sum of the deviations from its first value
-    float mean = g.sum(total, buf[0]) * inv;
-    float2 dev = make_float2(0.0f, 0.0f);
+    float mean = g.sum(total.x + total.y, buf[0]) * inv;
+    float2 dev1 = both(0.0f), dev2 = both(0.0f), minus = both(-mean);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
+      const int c = c0 + k * advance;
+      if (c < 0 || c + V > a.dim) {                 // what lies outside the row deviates by nothing
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        const float d = (EDGE ? (unsigned)(c + t) < (unsigned)a.dim : c < a.dim) ? v[k][t] - mean : 0.0f;
-        dev.x += d;
-        dev.y = __fmaf_rn(d, d, dev.y);
+        for (int t = 0; t < H; ++t) {
+          if ((unsigned)(c + 2 * t) >= (unsigned)a.dim) v[k][t].x = mean;
+          if ((unsigned)(c + 2 * t + 1) >= (unsigned)a.dim) v[k][t].y = mean;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < H; ++t) {
+        const float2 d = __fadd2_rn(v[k][t], minus);
+        dev1 = __fadd2_rn(dev1, d);
+        dev2 = __ffma2_rn(d, d, dev2);
       }
     }
-    dev = g.sum(dev, buf[1]);
+    const float2 dev = g.sum(make_float2(dev1.x + dev1.y, dev2.x + dev2.y), buf[1]);
     const float off = dev.x * inv;
     mean += off;
+    minus = both(-mean);
     const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
     if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+    T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
+      const int c = c0 + k * advance;
       if (c >= a.dim) continue;
-      uint32_t keep = 0xffffffffu;
-      if constexpr (DROP) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
-      float o[V];
+      float2 o[H];
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        float z = affine((v[k][t] - mean) * rstd, w[k][t], b[k][t]);
-        if (a.relu) z = relu_of(z);
-        if constexpr (DROP) z = (keep >> t) & 1 ? z * a.drop.scale : 0.0f;
-        o[t] = z;
+      for (int t = 0; t < H; ++t) o[t] = __ffma2_rn(__fmul2_rn(__fadd2_rn(v[k][t], minus), both(rstd)), w[k][t], b[k][t]);
+      if constexpr (HIDDEN) {
+        if (a.relu) {
+#pragma unroll
+          for (int t = 0; t < H; ++t) o[t] = make_float2(relu_of(o[t].x), relu_of(o[t].y));
+        }
+        if (a.drop.on) {
+          const uint32_t keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
+#pragma unroll
+          for (int t = 0; t < H; ++t) o[t] = select(keep, t, __fmul2_rn(o[t], both(a.drop.scale)));
+        }
       }
       store_vec<T, EDGE>(y, c, a.dim, o);
     }
@@ -270,7 +373,7 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256) norm_forward_kernel(const 
 // Sums the groups' column sums of a block in order and stores them: out[c] for c in [0, dim).  Group i holds its
 // vectors' elements in `acc`; its columns are shifted by shift(i).
 template <class T, int L, int C, bool EDGE>
-__device__ __forceinline__ void store_columns(const float (&acc)[C][kVec<T>], const Group<L>& g, float* out, int dim,
+__device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2], const Group<L>& g, float* out, int dim,
                                               const void* base, int64_t ld, float* smem) {
   constexpr int V = kVec<T>;
   if constexpr (L == 0) {
@@ -280,7 +383,7 @@ __device__ __forceinline__ void store_columns(const float (&acc)[C][kVec<T>], co
 #pragma unroll
       for (int t = 0; t < V; ++t) {
         const int c = (g.lane + k * g.lanes) * V - s + t;
-        if ((unsigned)c < (unsigned)dim) out[c] = acc[k][t];
+        if ((unsigned)c < (unsigned)dim) out[c] = half_of(acc[k][t / 2], t % 2);
       }
   } else {
     constexpr int kWidth = L * C * V, kGroups = 256 / L;
@@ -288,7 +391,7 @@ __device__ __forceinline__ void store_columns(const float (&acc)[C][kVec<T>], co
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
-      for (int t = 0; t < V; ++t) smem[g.index * kWidth + (g.lane + k * L) * V + t] = acc[k][t];
+      for (int t = 0; t < V; ++t) smem[g.index * kWidth + (g.lane + k * L) * V + t] = half_of(acc[k][t / 2], t % 2);
     __syncthreads();
     for (int c = threadIdx.x; c < dim; c += 256) {
       float sum = 0.0f;
@@ -301,81 +404,101 @@ __device__ __forceinline__ void store_columns(const float (&acc)[C][kVec<T>], co
 }
 
 // dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
-template <class T, int L, int C, bool DROP, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256) norm_backward_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int V = kVec<T>;
+template <class T, int L, int C, bool HIDDEN, bool EDGE>
+__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int V = kVec<T>, H = V / 2;
   __shared__ float2 buf[2][32];
-  extern __shared__ float columns[];
+  extern __shared__ uint4 ring_memory[];
   const Group<L> g;
   const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
-  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  int c0 = g.lane * V - s;
+  const int advance = g.lanes * V;
+  const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
   const float inv = 1.0f / (float)a.dim;
-  float w[C][V], b[C][V], aw[C][V], ab[C][V];
+  constexpr int S = ring_slots<C>();
+  const Ring<T, C, S, EDGE> ring_x(ring_memory, 0), ring_dy(ring_memory, 1);
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    const int64_t r = g.first + i * g.stride;
+    if (r < a.rows) {
+      ring_x.fetch(i, x + r * a.ldx, c0, advance, a.dim);
+      ring_dy.fetch(i, dy + r * a.lddy, c0, advance, a.dim);
+    }
+    copy_commit();
+  }
+  float2 st_next = g.first < a.rows ? a.stats[g.first] : both(0.0f);
+  float2 w[C][H], b[HIDDEN ? C : 1][H], aw[C][H], ab[C][H];
+  load_columns<T, C>(w, a.weight, a.wf32, a.dim, c0, advance, 1.0f);
+  if constexpr (HIDDEN) load_columns<T, C>(b, a.relu ? a.bias : nullptr, a.wf32, a.dim, c0, advance, 0.0f);
 #pragma unroll
   for (int k = 0; k < C; ++k)
 #pragma unroll
-    for (int t = 0; t < V; ++t) {
-      const int c = (g.lane + k * g.lanes) * V - s + t;
-      const bool in = (unsigned)c < (unsigned)a.dim;
-      w[k][t] = in && a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f;
-      b[k][t] = in && a.relu && a.bias != nullptr ? vector_at<T>(a.bias, a.wf32, c) : 0.0f;
-      aw[k][t] = ab[k][t] = 0.0f;
-    }
-  int turn = 0;
+    for (int t = 0; t < H; ++t) aw[k][t] = ab[k][t] = both(0.0f);
+  int turn = 0, slot = 0;
   for (int64_t r = g.first; r < a.rows; r += g.stride, turn ^= 1) {
-    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx;
-    const T* dy = reinterpret_cast<const T*>(a.dy) + r * a.lddy;
+    if constexpr (EDGE) not_hoisted(c0);
+    const float2 st = st_next;
+    if (r + g.stride < a.rows) st_next = a.stats[r + g.stride];
     Pack<T> rx[C], rd[C];
-#pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
-      if (c < a.dim) {
-        load_vec<T, EDGE>(rx[k], x, c, a.dim);
-        load_vec<T, EDGE>(rd[k], dy, c, a.dim);
-      } else {
-        rx[k].raw = rd[k].raw = make_uint4(0, 0, 0, 0);
-      }
+    copy_wait<S - 2>();
+    ring_x.read(slot, rx, c0);
+    ring_dy.read(slot, rd, c0);
+    const int64_t ahead = r + (S - 1) * g.stride;
+    if (ahead < a.rows) {
+      ring_x.fetch(slot == 0 ? S - 1 : slot - 1, x + ahead * a.ldx, c0, advance, a.dim);
+      ring_dy.fetch(slot == 0 ? S - 1 : slot - 1, dy + ahead * a.lddy, c0, advance, a.dim);
     }
-    const float2 st = a.stats[r];
-    float h[C][V], gr[C][V];
-    float2 sums = make_float2(0.0f, 0.0f);
+    copy_commit();
+    slot = slot == S - 1 ? 0 : slot + 1;
+    const float2 minus = both(-st.x), rstd = both(st.y);
+    float2 h[C][H], gr[C][H], s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
+      const int c = c0 + k * advance;
+      unpack<T>(rx[k], h[k]);
+      unpack<T>(rd[k], gr[k]);
       uint32_t keep = 0xffffffffu;
-      if constexpr (DROP) {
-        if (c < a.dim) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
+      if constexpr (HIDDEN) {
+        if (a.drop.on && c < a.dim) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
       }
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        // a column outside the row has dy = 0 and adds nothing anywhere
-        const bool in = EDGE ? (unsigned)(c + t) < (unsigned)a.dim : c < a.dim;
-        h[k][t] = in ? (to_float(rx[k].v[t]) - st.x) * st.y : 0.0f;
-        float dz = to_float(rd[k].v[t]);
-        if constexpr (DROP) dz = (keep >> t) & 1 ? dz * a.drop.scale : 0.0f;
-        if (a.relu && affine(h[k][t], w[k][t], b[k][t]) <= 0.0f) dz = 0.0f;
-        aw[k][t] = __fmaf_rn(dz, h[k][t], aw[k][t]);
-        ab[k][t] += dz;
-        gr[k][t] = dz * w[k][t];
-        sums.x += gr[k][t];
-        sums.y = __fmaf_rn(gr[k][t], h[k][t], sums.y);
+      for (int t = 0; t < H; ++t) {
+        // (a column outside the row has x = dy = 0 and adds nothing anywhere)
+        h[k][t] = __fmul2_rn(__fadd2_rn(h[k][t], minus), rstd);
+        float2 dz = gr[k][t];
+        if constexpr (HIDDEN) {
+          dz = select(keep, t, __fmul2_rn(dz, both(a.drop.scale)));
+          if (a.relu) {
+            const float2 z = __ffma2_rn(h[k][t], w[k][t], b[k][t]);
+            dz = make_float2(z.x <= 0.0f ? 0.0f : dz.x, z.y <= 0.0f ? 0.0f : dz.y);
+          }
+        }
+        aw[k][t] = __ffma2_rn(dz, h[k][t], aw[k][t]);
+        ab[k][t] = __fadd2_rn(ab[k][t], dz);
+        gr[k][t] = __fmul2_rn(dz, w[k][t]);
+        s1 = __fadd2_rn(s1, gr[k][t]);
+        s2 = __ffma2_rn(gr[k][t], h[k][t], s2);
       }
     }
     if (a.out == nullptr) continue;
     T* dx = reinterpret_cast<T*>(a.out) + r * a.ldo;
-    sums = g.sum(sums, buf[turn]);
-    const float c1 = sums.x * inv, c2 = sums.y * inv;
+    const float2 sums = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), buf[turn]);
+    const float2 c1 = both(-sums.x * inv), c2 = both(-sums.y * inv);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = (g.lane + k * g.lanes) * V - s;
+      const int c = c0 + k * advance;
       if (c >= a.dim) continue;
-      float o[V];
+      float2 o[H];
 #pragma unroll
-      for (int t = 0; t < V; ++t) o[t] = st.y * (gr[k][t] - __fmaf_rn(h[k][t], c2, c1));
+      for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(__fadd2_rn(gr[k][t], __ffma2_rn(h[k][t], c2, c1)), rstd);
       store_vec<T, EDGE>(dx, c, a.dim, o);
     }
   }
   if (a.partial != nullptr) {
+    copy_wait<0>();                                 // the groups' sums go where the ring was
+    float* columns = reinterpret_cast<float*>(ring_memory);
     float* p = a.partial + (int64_t)blockIdx.x * 2 * a.dim;
     store_columns<T, L, C, EDGE>(aw, g, p, a.dim, a.x, a.ldx, columns);
     store_columns<T, L, C, EDGE>(ab, g, p + a.dim, a.dim, a.x, a.ldx, columns);
@@ -499,21 +622,33 @@ __global__ void __launch_bounds__(128) norm_backward_columns_plain(const __grid_
 // the forward's output y says which elements were kept and positive
 template <class T, bool BACK, bool EDGE>
 __device__ __forceinline__ void drop_vec(const DropArgs& a, uint64_t step, int64_t e, const Pack<T>& in, const Pack<T>& y,
-                                         const float (&b)[kVec<T>], float (&o)[kVec<T>]) {
-  constexpr int V = kVec<T>;
+                                         const float2 (&b)[kVec<T> / 2], float2 (&o)[kVec<T> / 2]) {
+  constexpr int V = kVec<T>, H = V / 2;
   const bool draw = a.drop.on && !(BACK && a.relu);
   const uint32_t keep = draw ? keep_bits<V, EDGE>(a.drop, step, e) : 0xffffffffu;
+  unpack<T>(in, o);
+  if constexpr (BACK) {
+    if (a.relu) {
+      float2 f[H];
+      unpack<T>(y, f);
 #pragma unroll
-  for (int t = 0; t < V; ++t) {
-    float z = to_float(in.v[t]);
-    if constexpr (BACK) {
-      z = ((keep >> t) & 1) && !(a.relu && to_float(y.v[t]) <= 0.0f) ? z * a.drop.scale : 0.0f;
-    } else {
-      z += b[t];
-      if (a.relu) z = relu_of(z);
-      z = (keep >> t) & 1 ? z * a.drop.scale : 0.0f;
+      for (int t = 0; t < H; ++t) o[t] = make_float2(f[t].x <= 0.0f ? 0.0f : o[t].x, f[t].y <= 0.0f ? 0.0f : o[t].y);
     }
-    o[t] = z;
+  } else {
+#pragma unroll
+    for (int t = 0; t < H; ++t) o[t] = __fadd2_rn(o[t], b[t]);
+    if (a.relu) {
+#pragma unroll
+      for (int t = 0; t < H; ++t) o[t] = make_float2(relu_of(o[t].x), relu_of(o[t].y));
+    }
+  }
+  if (a.drop.on) {
+#pragma unroll
+    for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(o[t], both(a.drop.scale));
+    if (draw) {
+#pragma unroll
+      for (int t = 0; t < H; ++t) o[t] = select(keep, t, o[t]);
+    }
   }
 }
 
@@ -526,7 +661,7 @@ __global__ void __launch_bounds__(256) dropout_flat_kernel(const __grid_constant
   const T* y = reinterpret_cast<const T*>(a.y);
   T* out = reinterpret_cast<T*>(a.out);
   const bool two = BACK && a.relu;
-  const float zero[V] = {};
+  const float2 zero[V / 2] = {};
   const int64_t vectors = n / V, stride = (int64_t)gridDim.x * 256;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vectors; i += U * stride) {
     Pack<T> in[U], yy[U];
@@ -539,13 +674,10 @@ __global__ void __launch_bounds__(256) dropout_flat_kernel(const __grid_constant
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i + u * stride < vectors) {
-        float o[V];
+        float2 o[V / 2];
         const int64_t e = (i + u * stride) * V;
         drop_vec<T, BACK, EDGE>(a, step, a.drop.first + e, in[u], yy[u], zero, o);
-        Pack<T> p;
-#pragma unroll
-        for (int t = 0; t < V; ++t) p.v[t] = from_float<T>(o[t]);
-        reinterpret_cast<uint4*>(out)[i + u * stride] = p.raw;
+        store_vec<T, false>(out + e, 0, V, o);
       }
   }
   // the last elements that fill no vector
@@ -571,12 +703,10 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
   const bool live = group < groups && c < a.dim;
   const uint64_t step = step_of(a.drop);
   const bool two = BACK && a.relu;
-  float b[V], acc[V];
+  float2 b[1][V / 2], acc[V / 2];
+  load_columns<T, 1>(b, !BACK && live ? a.bias : nullptr, a.bf32, a.dim, c, 0, 0.0f);
 #pragma unroll
-  for (int t = 0; t < V; ++t) {
-    b[t] = !BACK && live && a.bias != nullptr && (unsigned)(c + t) < (unsigned)a.dim ? vector_at<T>(a.bias, a.bf32, c + t) : 0.0f;
-    acc[t] = 0.0f;
-  }
+  for (int t = 0; t < V / 2; ++t) acc[t] = both(0.0f);
   if (live) {
     for (int64_t r = first; r < a.rows; r += U * stride) {
       Pack<T> in[U], yy[U];
@@ -589,11 +719,11 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + u * stride < a.rows) {
-          float o[V];
-          drop_vec<T, BACK, EDGE>(a, step, a.drop.first + (r + u * stride) * a.dim + c, in[u], yy[u], b, o);
+          float2 o[V / 2];
+          drop_vec<T, BACK, EDGE>(a, step, a.drop.first + (r + u * stride) * a.dim + c, in[u], yy[u], b[0], o);
           if constexpr (BACK) {
 #pragma unroll
-            for (int t = 0; t < V; ++t) acc[t] += o[t];
+            for (int t = 0; t < V / 2; ++t) acc[t] = __fadd2_rn(acc[t], o[t]);
           }
           if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o);
         }
@@ -602,7 +732,7 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
   if (!BACK || a.partial == nullptr) return;
   if (group < groups) {
 #pragma unroll
-    for (int t = 0; t < V; ++t) columns[(group * a.lanes + lane) * V + t] = live ? acc[t] : 0.0f;
+    for (int t = 0; t < V; ++t) columns[(group * a.lanes + lane) * V + t] = live ? half_of(acc[t / 2], t % 2) : 0.0f;
   }
   __syncthreads();
   const int tile = a.lanes * V, c0 = blockIdx.y * tile;
@@ -693,6 +823,17 @@ Layout layout_of(int64_t rows, int dim, std::initializer_list<Matrix> all) {
   return {true, dim % V != 0 || shift != 0, (int)(((int64_t)dim + shift + V - 1) / V)};
 }
 
+// Lets a kernel have `smem` bytes of dynamic shared memory (and its static ones: 48 KB together need no leave) on the current
+// device; `done`: a bit per device that was seen.
+template <class K>
+void allow_smem(K kernel, int smem, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (smem <= 46 << 10 || cudaGetDevice(&device) != cudaSuccess) return;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <class K>
 int blocks_per_sm(K kernel, int threads, int smem) {
   int n = 0;
@@ -701,58 +842,82 @@ int blocks_per_sm(K kernel, int threads, int smem) {
 
 inline int clamp_blocks(int64_t wanted, int64_t most) { return (int)std::max<int64_t>(1, std::min(wanted, most)); }
 
-// group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads)
+// a block per row
+template <int C, class F>
+bool wide_rows(int vectors, F&& f) {
+  const int threads = ((vectors + C - 1) / C + 31) / 32 * 32;
+  if (threads > 512) return false;
+  f.template operator()<0, C>(threads);
+  return true;
+}
+
+// Group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads).  The
+// fewest lanes whose registers hold the row: they have the most bytes in flight each and the fewest steps in the row's sums.
 template <class T, class F>
 bool by_width(int vectors, F&& f) {
-  constexpr bool wide = sizeof(T) == 4;          // 16 (20) elements per thread either way
-  if (vectors <= 4) f.template operator()<4, 1>(256);
-  else if (vectors <= 8) f.template operator()<8, 1>(256);
-  else if (vectors <= 16) f.template operator()<16, 1>(256);
-  else if (vectors <= 32) f.template operator()<32, 1>(256);
-  else if (vectors <= 64) f.template operator()<32, 2>(256);
-  else if (wide && vectors <= 96) f.template operator()<32, wide ? 3 : 2>(256);
-  else if (wide && vectors <= 128) f.template operator()<32, wide ? 4 : 2>(256);
-  else if (wide && vectors <= 160) f.template operator()<32, wide ? 5 : 2>(256);
-  else {
-    constexpr int C = wide ? 4 : 2;
-    const int threads = ((vectors + C - 1) / C + 31) / 32 * 32;
-    if (threads > 512) return false;
-    f.template operator()<0, C>(threads);
+  if constexpr (sizeof(T) == 4) {                // up to 20 elements per thread
+    if (vectors <= 4) f.template operator()<4, 1>(256);
+    else if (vectors <= 8) f.template operator()<4, 2>(256);
+    else if (vectors <= 12) f.template operator()<4, 3>(256);
+    else if (vectors <= 16) f.template operator()<4, 4>(256);
+    else if (vectors <= 20) f.template operator()<4, 5>(256);
+    else if (vectors <= 24) f.template operator()<8, 3>(256);
+    else if (vectors <= 32) f.template operator()<8, 4>(256);
+    else if (vectors <= 40) f.template operator()<8, 5>(256);
+    else if (vectors <= 48) f.template operator()<16, 3>(256);
+    else if (vectors <= 64) f.template operator()<16, 4>(256);
+    else if (vectors <= 80) f.template operator()<16, 5>(256);
+    else if (vectors <= 96) f.template operator()<32, 3>(256);
+    else if (vectors <= 128) f.template operator()<32, 4>(256);
+    else if (vectors <= 160) f.template operator()<32, 5>(256);
+    else return wide_rows<4>(vectors, f);
+  } else {                                       // up to 16
+    if (vectors <= 4) f.template operator()<4, 1>(256);
+    else if (vectors <= 8) f.template operator()<4, 2>(256);
+    else if (vectors <= 16) f.template operator()<8, 2>(256);
+    else if (vectors <= 32) f.template operator()<16, 2>(256);
+    else if (vectors <= 64) f.template operator()<32, 2>(256);
+    else return wide_rows<2>(vectors, f);
   }
   return true;
 }
 
-template <class T, bool DROP, bool EDGE>
+template <class T, bool HIDDEN, bool EDGE>
 struct NormForward {
   const NormArgs& a;
   cudaStream_t stream;
   template <int L, int C>
   void operator()(int threads) const {
-    auto kernel = norm_forward_kernel<T, L, C, DROP, EDGE>;
-    static const int full = blocks_per_sm(kernel, L == 0 ? 256 : 256, 0);
+    auto kernel = norm_forward_kernel<T, L, C, HIDDEN, EDGE>;
+    constexpr int per_thread = 16 * C * ring_slots<C>();
+    static std::atomic<uint64_t> seen{0};
+    allow_smem(kernel, per_thread * (L == 0 ? 512 : 256), seen);
+    static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
     constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
     int64_t most = (int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full);
     int blocks = clamp_blocks((a.rows + per - 1) / per, most);
     if (L == 0) blocks = (blocks + 7) / 8 * 8;
-    kernel<<<blocks, threads, 0, stream>>>(a);
+    kernel<<<blocks, threads, per_thread * threads, stream>>>(a);
   }
 };
 
-template <class T, bool DROP, bool EDGE>
+template <class T, bool HIDDEN, bool EDGE>
 struct NormBackward {
   const NormArgs& a;
   cudaStream_t stream;
   int* blocks;
   template <int L, int C>
   void operator()(int threads) const {
-    auto kernel = norm_backward_kernel<T, L, C, DROP, EDGE>;
-    constexpr int smem = L == 0 ? 0 : 256 * C * kVec<T> * 4;
-    static const int full = blocks_per_sm(kernel, 256, smem);
+    auto kernel = norm_backward_kernel<T, L, C, HIDDEN, EDGE>;
+    constexpr int per_thread = std::max(32 * C * ring_slots<C>(), L == 0 ? 0 : C * kVec<T> * 4);
+    static std::atomic<uint64_t> seen{0};
+    allow_smem(kernel, per_thread * (L == 0 ? 512 : 256), seen);
+    static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
     constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
     const int64_t most = std::min<int64_t>((int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full), column_blocks_cap(a.rows, a.dim));
     *blocks = clamp_blocks((a.rows + per - 1) / per, most);
     if (L == 0) *blocks = *blocks < 8 ? 8 : *blocks / 8 * 8;
-    kernel<<<*blocks, threads, smem, stream>>>(a);
+    kernel<<<*blocks, threads, per_thread * threads, stream>>>(a);
   }
 };
 
@@ -774,7 +939,7 @@ cudaError_t launch_norm_forward(const NormArgs& given, cudaStream_t stream) {
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
   bool done = false;
   if (l.vec) {
-    if (a.drop.on) done = l.edge ? by_width<T>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, true, false>{a, stream});
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, true, false>{a, stream});
     else done = l.edge ? by_width<T>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, false, false>{a, stream});
   }
   if (!done) norm_forward_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
@@ -788,7 +953,7 @@ cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
   bool done = false;
   if (l.vec) {
-    if (a.drop.on) done = l.edge ? by_width<T>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
     else done = l.edge ? by_width<T>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
   }
   if (!done) {

@@ -12,12 +12,9 @@ reads the tensor too: change it after the backward pass only (in eager mode auto
 All sums and statistics are held in 32 bits whatever the matrix's type (float32, bfloat16, float16); results
 are rounded once and are the same bit for bit on every call.  As everywhere in this package there is no CPU path.
 """
-import ctypes
-
 import torch
 
 from . import _native
-from .plan import _device_guard
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -40,7 +37,7 @@ def _check_vector(v, name, x):
         raise TypeError(f"{name} must be a torch.Tensor")
     if v.device != x.device or v.dim() != 1 or v.size(0) != x.size(-1):
         raise RuntimeError(f"{name} must be a vector of {x.size(-1)} entries on x's device, got {tuple(v.shape)} on {v.device}")
-    if v.dtype not in (torch.float32, x.dtype):
+    if v.dtype is not torch.float32 and v.dtype is not x.dtype:
         raise RuntimeError(f"{name} must be float32 or of x's type, got {v.dtype}")
 
 
@@ -74,53 +71,97 @@ def _check_drop(p, seed, step, row_offset, training, x):
 def _rows(x):
     """x as [rows, width] with unit column stride: a view where its layout allows it, else a copy"""
     v = x if x.dim() == 2 else x.unsqueeze(0) if x.dim() == 1 else x.flatten(0, -2)
-    if (v.stride(1) == 1 or v.size(1) <= 1) and (v.stride(0) >= v.size(1) or v.size(0) <= 1):
+    if v.is_contiguous() or ((v.stride(1) == 1 or v.size(1) <= 1) and (v.stride(0) >= v.size(1) or v.size(0) <= 1)):
         return v
     return v.contiguous()
 
 
-def _ld(x):
-    return x.stride(0) if x.size(0) > 1 else x.size(1)
-
-
-def _drop_arg(drop):
+def _drop_arg(drop, step):
     if drop is None:
         return None
-    p, seed, step, tensor, row_offset = drop
-    return _native.Dropout(p, seed, step, tensor.data_ptr() if tensor is not None else None, row_offset)
+    return _native.Dropout(drop[0], drop[1], drop[2], step.data_ptr() if step is not None else None, drop[4])
 
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _kind(weight, bias, x):
+    """the one type in which both vectors go down: their own, or 32-bit where they differ"""
+    if weight is None or bias is None:
+        v = bias if weight is None else weight
+        return torch.float32 if v is None else v.dtype
+    return weight.dtype if weight.dtype is bias.dtype else torch.float32
 
 
-def _vectors(weight, bias, x):
-    """contiguous vectors of one type -> (weight, bias, type code)"""
-    kinds = {v.dtype for v in (weight, bias) if v is not None}
-    kind = kinds.pop() if len(kinds) == 1 else torch.float32
-    weight, bias = (v if v is None else v.to(kind).contiguous() for v in (weight, bias))
-    return weight, bias, DTYPES[kind]
+def _vector(v, kind):
+    if v is None or (v.dtype is kind and v.is_contiguous()):
+        return v
+    return v.to(kind).contiguous()
 
 
-def _workspace(rows, width, device):
+def _call(function, x, *args):
+    """a C-ABI call that enqueues on the current stream of x's device"""
+    index = x.get_device()
+    if index == torch.cuda.current_device():
+        _native.check(function(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _native.check(function(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _workspace(lib, rows, width, x):
     # torch's caching allocator returns 512-byte aligned blocks
-    return torch.empty(int(_native.cuda().rof_layer_norm_workspace_bytes(rows, width)), dtype=torch.uint8, device=device)
+    n = lib.rof_layer_norm_workspace_bytes(rows, width)
+    return torch.empty(n, dtype=torch.uint8, device=x.device), n
 
 
 def _norm_forward(x, weight, bias, eps, relu, drop, want_stats):
     v = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((v.size(0), 2), dtype=torch.float32, device=x.device) if want_stats else None
-    weight, bias, kind = _vectors(weight, bias, x)
-    with _device_guard(x.device):
-        _native.check(_native.cuda().rof_layer_norm_forward(
-            DTYPES[x.dtype], v.data_ptr(), _ld(v), v.size(0), v.size(1), kind, _ptr(weight), _ptr(bias), eps, int(relu),
-            _drop_arg(drop), y.data_ptr(), v.size(1), _ptr(stats), _stream(x.device)))
+    rows, width = v.shape
+    y = _like(x)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if want_stats else None
+    kind = _kind(weight, bias, x)
+    w, b = _vector(weight, kind), _vector(bias, kind)
+    _call(_native.cuda().rof_layer_norm_forward, x, DTYPES[x.dtype], v.data_ptr(), v.stride(0), rows, width, DTYPES[kind],
+          _ptr(w), _ptr(b), eps, relu, _drop_arg(drop, drop[3] if drop else None), y.data_ptr(), width, _ptr(stats))
     return v, y, stats
+
+
+def _norm_backward(ctx, grad):
+    v, weight, bias, stats, step = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    rows, width = v.shape
+    dy = _rows(grad)
+    dx = _like(grad) if need_x else None
+    kind = _kind(weight, bias, v)
+    w, b = _vector(weight, kind), _vector(bias, kind)
+    dw = _like(w) if need_w else None
+    db = _like(b) if need_b else None
+    lib = _native.cuda()
+    ws, n = _workspace(lib, rows, width, v) if need_w or need_b else (None, 0)
+    _call(lib.rof_layer_norm_backward, v, DTYPES[v.dtype], dy.data_ptr(), dy.stride(0), v.data_ptr(), v.stride(0), rows, width,
+          DTYPES[kind], _ptr(w), _ptr(b), stats.data_ptr(), ctx.relu, _drop_arg(ctx.drop, step), _ptr(dx), width,
+          _ptr(dw), _ptr(db), _ptr(ws), n)
+    if need_w and dw.dtype is not weight.dtype:
+        dw = dw.to(weight.dtype)
+    if need_b and db.dtype is not bias.dtype:
+        db = db.to(bias.dtype)
+    return dx, dw, db, None, None, None, None
+
+
+# The wrapper that refuses a second derivative costs 12 us a call: it is only gone through where a graph of the
+# gradients is being made (create_graph).
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
+
+
+def _without_tensor(drop):
+    """what the autograd node keeps of a drop: the step tensor is saved apart, where changes to it are seen"""
+    return drop[:3] + (None, drop[4]) if drop is not None else None
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -128,30 +169,12 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, relu, drop, step):
         v, y, stats = _norm_forward(x, weight, bias, eps, relu, drop, True)
         ctx.save_for_backward(v, weight, bias, stats, step)
-        ctx.relu, ctx.drop, ctx.shape = relu, drop[:3] + drop[4:] if drop else None, x.shape
+        ctx.relu, ctx.drop = relu, _without_tensor(drop)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        v, weight, bias, stats, step = ctx.saved_tensors
-        drop = ctx.drop[:3] + (step,) + ctx.drop[3:] if ctx.drop else None
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        rows, width = v.shape
-        dy = _rows(grad)
-        dx = torch.empty(ctx.shape, dtype=v.dtype, device=v.device) if need_x else None
-        w, b, kind = _vectors(weight, bias, v)
-        like = w if w is not None else b
-        dw = torch.empty_like(like) if need_w else None
-        db = torch.empty_like(like) if need_b else None
-        ws = _workspace(rows, width, v.device) if need_w or need_b else None
-        with _device_guard(v.device):
-            _native.check(_native.cuda().rof_layer_norm_backward(
-                DTYPES[v.dtype], dy.data_ptr(), _ld(dy), v.data_ptr(), _ld(v), rows, width, kind, _ptr(w), _ptr(b),
-                stats.data_ptr(), int(ctx.relu), _drop_arg(drop), _ptr(dx), width, _ptr(dw), _ptr(db), _ptr(ws),
-                ws.numel() if ws is not None else 0, _stream(v.device)))
-        return (dx, dw.to(weight.dtype) if need_w else None,
-                db.to(bias.dtype) if need_b else None, None, None, None, None)
+        return _norm_backward_once(ctx, grad) if torch.is_grad_enabled() else _norm_backward(ctx, grad)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None, step=0, row_offset=0, training=True):
@@ -167,20 +190,41 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     drop = _check_drop(p, seed, step, row_offset, training, x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNorm.apply(x, weight, bias, float(eps), bool(relu), drop, drop[3] if drop else None)
-    return _norm_forward(x, weight, bias, float(eps), bool(relu), drop, False)[1]
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps, bool(relu), drop, drop[3] if drop else None)
+    return _norm_forward(x, weight, bias, eps, bool(relu), drop, False)[1]
 
 
 def _dropout_forward(x, bias, relu, drop):
     v = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _, bias, kind = _vectors(None, bias, x)
-    with _device_guard(x.device):
-        _native.check(_native.cuda().rof_dropout_forward(
-            DTYPES[x.dtype], v.data_ptr(), _ld(v), v.size(0), v.size(1), kind, _ptr(bias), int(relu), _drop_arg(drop),
-            y.data_ptr(), v.size(1), _stream(x.device)))
+    rows, width = v.shape
+    y = _like(x)
+    kind = torch.float32 if bias is None else bias.dtype
+    b = _vector(bias, kind)
+    _call(_native.cuda().rof_dropout_forward, x, DTYPES[x.dtype], v.data_ptr(), v.stride(0), rows, width, DTYPES[kind], _ptr(b),
+          relu, _drop_arg(drop, drop[3] if drop else None), y.data_ptr(), width)
     return y
+
+
+def _dropout_backward(ctx, grad):
+    y, step = ctx.saved_tensors
+    need_x, need_b = ctx.needs_input_grad[:2]
+    dy = _rows(grad)
+    rows, width = dy.shape
+    dx = _like(grad) if need_x else None
+    kind = ctx.bias_kind
+    lib = _native.cuda()
+    db, (ws, n) = None, (None, 0)
+    if need_b:
+        db = torch.empty(width, dtype=kind, device=dy.device)
+        ws, n = _workspace(lib, rows, width, dy)
+    _call(lib.rof_dropout_backward, dy, DTYPES[dy.dtype], dy.data_ptr(), dy.stride(0), _ptr(y), width, rows, width, DTYPES[kind],
+          ctx.relu, _drop_arg(ctx.drop, step), _ptr(dx), width, _ptr(db), _ptr(ws), n)
+    return dx, db, None, None, None
+
+
+_dropout_backward_once = torch.autograd.function.once_differentiable(_dropout_backward)
 
 
 class _Dropout(torch.autograd.Function):
@@ -189,27 +233,13 @@ class _Dropout(torch.autograd.Function):
         y = _dropout_forward(x, bias, relu, drop)
         # behind a ReLU the output says which elements were kept and positive
         ctx.save_for_backward(y if relu else None, step)
-        ctx.relu, ctx.drop = relu, drop[:3] + drop[4:] if drop else None
-        ctx.bias_kind = bias.dtype if bias is not None else None
+        ctx.relu, ctx.drop = relu, _without_tensor(drop)
+        ctx.bias_kind = bias.dtype if bias is not None else torch.float32
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        y, step = ctx.saved_tensors
-        drop = ctx.drop[:3] + (step,) + ctx.drop[3:] if ctx.drop else None
-        need_x, need_b = ctx.needs_input_grad[:2]
-        dy = _rows(grad)
-        rows, width = dy.shape
-        dx = torch.empty(grad.shape, dtype=dy.dtype, device=dy.device) if need_x else None
-        db = torch.empty(width, dtype=ctx.bias_kind, device=dy.device) if need_b else None
-        ws = _workspace(rows, width, dy.device) if need_b else None
-        with _device_guard(dy.device):
-            _native.check(_native.cuda().rof_dropout_backward(
-                DTYPES[dy.dtype], dy.data_ptr(), _ld(dy), _ptr(y), width, rows, width,
-                DTYPES[ctx.bias_kind] if need_b else 0, int(ctx.relu), _drop_arg(drop), _ptr(dx), width, _ptr(db), _ptr(ws),
-                ws.numel() if ws is not None else 0, _stream(dy.device)))
-        return dx, db, None, None, None
+        return _dropout_backward_once(ctx, grad) if torch.is_grad_enabled() else _dropout_backward(ctx, grad)
 
 
 def dropout(x, p=0.0, seed=None, step=0, row_offset=0, training=True, bias=None, relu=False):
