@@ -146,32 +146,38 @@ __device__ __forceinline__ bool kept(const Drop& d, uint64_t step, int64_t e) {
   return word(philox7((uint64_t)e >> 2, step, d.k0, d.k1), (int)(e & 3)) > d.last;
 }
 
-// bit t: element e + t stays (N a multiple of 4).  One Philox call gives the words of four elements that start at a multiple of
-// four; elsewhere (EDGE only) the N elements lie in N / 4 + 1 such groups.
+// v[t] = element e + t stays ? v[t] : 0 for N elements, N a multiple of 4.  One Philox call gives the words of four elements that
+// start at a multiple of four.  Elsewhere (EDGE only) the elements lie in N / 4 + 1 such groups; their words are moved into
+// place first, a path of rows with a stride or an offset of their own.
 template <int N, bool EDGE>
-__device__ __forceinline__ uint32_t keep_bits(const Drop& d, uint64_t step, int64_t e) {
+__device__ __forceinline__ void drop_elements(const Drop& d, uint64_t step, int64_t e, float2 (&v)[N / 2]) {
   const int sh = EDGE ? (int)(e & 3) : 0;
-  uint32_t bits = 0;
+  if (!EDGE || sh == 0) {
 #pragma unroll
-  for (int q = 0; q < N / 4; ++q) {
-    const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
-    bits |= (uint32_t)(w.x > d.last) << (4 * q);
-    bits |= (uint32_t)(w.y > d.last) << (4 * q + 1);
-    bits |= (uint32_t)(w.z > d.last) << (4 * q + 2);
-    bits |= (uint32_t)(w.w > d.last) << (4 * q + 3);
-  }
-  if (EDGE && sh != 0) {
-    const uint4 w = philox7((uint64_t)(e >> 2) + N / 4, step, d.k0, d.k1);
-    bits |= (uint32_t)(w.x > d.last) << N;
-    bits |= (uint32_t)(w.y > d.last) << (N + 1);
-    bits |= (uint32_t)(w.z > d.last) << (N + 2);
+    for (int q = 0; q < N / 4; ++q) {
+      const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
+      v[2 * q].x = w.x > d.last ? v[2 * q].x : 0.0f;
+      v[2 * q].y = w.y > d.last ? v[2 * q].y : 0.0f;
+      v[2 * q + 1].x = w.z > d.last ? v[2 * q + 1].x : 0.0f;
+      v[2 * q + 1].y = w.w > d.last ? v[2 * q + 1].y : 0.0f;
+    }
+  } else {
+    uint32_t bits = 0;
+    for (int q = 0; q <= N / 4; ++q) {
+      const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
+      bits |= ((uint32_t)(w.x > d.last) | (uint32_t)(w.y > d.last) << 1 | (uint32_t)(w.z > d.last) << 2 | (uint32_t)(w.w > d.last) << 3) << (4 * q);
+    }
     bits >>= sh;
+#pragma unroll
+    for (int t = 0; t < N / 2; ++t) v[t] = make_float2((bits >> (2 * t)) & 1 ? v[t].x : 0.0f, (bits >> (2 * t + 1)) & 1 ? v[t].y : 0.0f);
   }
-  return bits;
 }
 
 // relu(z) and its gradient keep a NaN, as torch's do
-__device__ __forceinline__ float relu_of(float z) { return z <= 0.0f ? 0.0f : z; }
+__device__ __forceinline__ float relu_of(float z) {
+  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z));
+  return z;
+}
 
 __device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
 
@@ -210,33 +216,45 @@ struct Group {
       stride = (int64_t)gridDim.x * (blockDim.x / L);
     }
   }
-  // sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
-  // for each of two sums that follow one another (L = 0 only)
-  __device__ __forceinline__ float2 sum(float2 v, float2* buf) const {
+  // Sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
+  // for each of two sums that follow one another (L = 0 only).
+  __device__ __forceinline__ float sum(float v, float* buf) const {
 #pragma unroll
-    for (int o = (L == 0 ? 32 : L) / 2; o > 0; o >>= 1) {
-      v.x += __shfl_xor_sync(mask, v.x, o);
-      v.y += __shfl_xor_sync(mask, v.y, o);
-    }
+    for (int o = (L == 0 ? 32 : L) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     if constexpr (L == 0) {
-      if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = buf[0];
-      for (int i = 1; i < (int)(blockDim.x >> 5); ++i) {
-        v.x += buf[i].x;
-        v.y += buf[i].y;
+      const int warps = blockDim.x >> 5;
+      if (warps > 1) {
+        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = (threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)              // at most 16 warps
+          if (o < warps) v += __shfl_xor_sync(mask, v, o);
+        v = __shfl_sync(mask, v, 0);
       }
     }
     return v;
   }
-  __device__ __forceinline__ float sum(float v, float2* buf) const {
-    if constexpr (L == 0) {
-      return sum(make_float2(v, 0.0f), buf).x;
-    } else {
+  // two sums at once: the first exchange leaves one of them to each half of the group
+  __device__ __forceinline__ float2 sum(float2 v, float* buf) const {
+    constexpr int W = L == 0 ? 32 : L;
+    const bool upper = threadIdx.x & (W / 2);
+    const float other = __shfl_xor_sync(mask, upper ? v.x : v.y, W / 2);
+    float mine = (upper ? v.y : v.x) + other;
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-      return v;
+    for (int o = W / 4; o > 0; o >>= 1) mine += __shfl_xor_sync(mask, mine, o);
+    if constexpr (L == 0) {
+      const int warps = blockDim.x >> 5, l = threadIdx.x & 31;
+      if (warps > 1) {
+        if ((threadIdx.x & 15) == 0) buf[(l >> 4) * 16 + (threadIdx.x >> 5)] = mine;
+        __syncthreads();
+        mine = (l & 15) < warps ? buf[l] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+          if (o < warps) mine += __shfl_xor_sync(mask, mine, o);
+      }
     }
+    return make_float2(__shfl_sync(mask, mine, 0, W), __shfl_sync(mask, mine, W / 2, W));
   }
 };
 
@@ -270,11 +288,6 @@ __device__ __forceinline__ void load_columns(float2 (&out)[C][kVec<T> / 2], cons
     }
 }
 
-// bits 2t and 2t + 1 of `keep` choose between v and zero
-__device__ __forceinline__ float2 select(uint32_t keep, int t, float2 v) {
-  return make_float2((keep >> (2 * t)) & 1 ? v.x : 0.0f, (keep >> (2 * t + 1)) & 1 ? v.y : 0.0f);
-}
-
 // What is computed from v is computed where it is used: the comparisons of a thread's columns with the ends of the row do not
 // change from row to row, but kept over the loop they cost more registers than the row itself.
 __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v)); }
@@ -283,7 +296,7 @@ __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v))
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
 __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
-  __shared__ float2 buf[2][32];
+  __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
   const Group<L> g;
   const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
@@ -360,9 +373,9 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
           for (int t = 0; t < H; ++t) o[t] = make_float2(relu_of(o[t].x), relu_of(o[t].y));
         }
         if (a.drop.on) {
-          const uint32_t keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
 #pragma unroll
-          for (int t = 0; t < H; ++t) o[t] = select(keep, t, __fmul2_rn(o[t], both(a.drop.scale)));
+          for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(o[t], both(a.drop.scale));
+          drop_elements<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c, o);
         }
       }
       store_vec<T, EDGE>(y, c, a.dim, o);
@@ -407,7 +420,7 @@ __device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
 __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
-  __shared__ float2 buf[2][32];
+  __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
   const Group<L> g;
   const int s = row_shift<T, EDGE>(a.x, a.ldx, g.first);
@@ -459,9 +472,12 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
       const int c = c0 + k * advance;
       unpack<T>(rx[k], h[k]);
       unpack<T>(rd[k], gr[k]);
-      uint32_t keep = 0xffffffffu;
       if constexpr (HIDDEN) {
-        if (a.drop.on && c < a.dim) keep = keep_bits<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c);
+        if (a.drop.on && c < a.dim) {
+#pragma unroll
+          for (int t = 0; t < H; ++t) gr[k][t] = __fmul2_rn(gr[k][t], both(a.drop.scale));
+          drop_elements<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c, gr[k]);
+        }
       }
 #pragma unroll
       for (int t = 0; t < H; ++t) {
@@ -469,7 +485,6 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
         h[k][t] = __fmul2_rn(__fadd2_rn(h[k][t], minus), rstd);
         float2 dz = gr[k][t];
         if constexpr (HIDDEN) {
-          dz = select(keep, t, __fmul2_rn(dz, both(a.drop.scale)));
           if (a.relu) {
             const float2 z = __ffma2_rn(h[k][t], w[k][t], b[k][t]);
             dz = make_float2(z.x <= 0.0f ? 0.0f : dz.x, z.y <= 0.0f ? 0.0f : dz.y);
@@ -531,7 +546,7 @@ __global__ void __launch_bounds__(256) join_columns_kernel(const float* partial,
 // wider than a block's registers; the row is read again instead of kept.
 template <class T>
 __global__ void __launch_bounds__(256) norm_forward_plain(const __grid_constant__ NormArgs a) {
-  __shared__ float2 buf[2][32];
+  __shared__ float buf[2][32];
   const Group<0> g;
   const uint64_t step = step_of(a.drop);
   const float inv = 1.0f / (float)a.dim;
@@ -572,7 +587,7 @@ __device__ __forceinline__ float norm_dz(const NormArgs& a, uint64_t step, int64
 
 template <class T>
 __global__ void __launch_bounds__(256) norm_backward_rows_plain(const __grid_constant__ NormArgs a) {
-  __shared__ float2 buf[2][32];
+  __shared__ float buf[2][32];
   const Group<0> g;
   const uint64_t step = step_of(a.drop);
   const float inv = 1.0f / (float)a.dim;
@@ -624,8 +639,6 @@ template <class T, bool BACK, bool EDGE>
 __device__ __forceinline__ void drop_vec(const DropArgs& a, uint64_t step, int64_t e, const Pack<T>& in, const Pack<T>& y,
                                          const float2 (&b)[kVec<T> / 2], float2 (&o)[kVec<T> / 2]) {
   constexpr int V = kVec<T>, H = V / 2;
-  const bool draw = a.drop.on && !(BACK && a.relu);
-  const uint32_t keep = draw ? keep_bits<V, EDGE>(a.drop, step, e) : 0xffffffffu;
   unpack<T>(in, o);
   if constexpr (BACK) {
     if (a.relu) {
@@ -645,10 +658,7 @@ __device__ __forceinline__ void drop_vec(const DropArgs& a, uint64_t step, int64
   if (a.drop.on) {
 #pragma unroll
     for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(o[t], both(a.drop.scale));
-    if (draw) {
-#pragma unroll
-      for (int t = 0; t < H; ++t) o[t] = select(keep, t, o[t]);
-    }
+    if (!(BACK && a.relu)) drop_elements<V, EDGE>(a.drop, step, e, o);
   }
 }
 
@@ -871,12 +881,16 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 128) f.template operator()<32, 4>(256);
     else if (vectors <= 160) f.template operator()<32, 5>(256);
     else return wide_rows<4>(vectors, f);
-  } else {                                       // up to 16
+  } else {                                       // up to 24
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<4, 2>(256);
+    else if (vectors <= 12) f.template operator()<4, 3>(256);
     else if (vectors <= 16) f.template operator()<8, 2>(256);
+    else if (vectors <= 24) f.template operator()<8, 3>(256);
     else if (vectors <= 32) f.template operator()<16, 2>(256);
+    else if (vectors <= 48) f.template operator()<16, 3>(256);
     else if (vectors <= 64) f.template operator()<32, 2>(256);
+    else if (vectors <= 96) f.template operator()<32, 3>(256);
     else return wide_rows<2>(vectors, f);
   }
   return true;
