@@ -1,0 +1,269 @@
+// Device code that the kernels of layer norm and dropout share: types, 16-byte vectors, asynchronous copies, the
+// generator, sums over a group of threads.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <initializer_list>
+
+#include "norm.h"
+
+namespace rof {
+namespace {
+
+// ---- types --------------------------------------------------------------------------------------
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+template <class T> constexpr int kVec = 16 / (int)sizeof(T);
+
+// a weight or bias vector: 32-bit, or of the matrix's own type
+template <class T>
+__device__ __forceinline__ float vector_at(const void* p, int f32, int i) {
+  return f32 ? __ldg(reinterpret_cast<const float*>(p) + i) : to_float(reinterpret_cast<const T*>(p)[i]);
+}
+
+template <class T>
+__device__ __forceinline__ void vector_put(void* p, int f32, int i, float v) {
+  if (f32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<T*>(p)[i] = from_float<T>(v);
+}
+
+template <class T>
+union Pack {
+  uint4 raw;
+  T v[kVec<T>];
+  __device__ Pack() {}
+};
+
+// columns [c, c + VEC) of a row; what lies outside [0, dim) is zero
+template <class T, bool EDGE>
+__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim) {
+  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
+    out.raw = *reinterpret_cast<const uint4*>(row + c);
+  } else {
+#pragma unroll
+    for (int t = 0; t < kVec<T>; ++t) out.v[t] = (unsigned)(c + t) < (unsigned)dim ? row[c + t] : from_float<T>(0.0f);
+  }
+}
+
+__device__ __forceinline__ void pack_two(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+__device__ __forceinline__ void pack_two(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void pack_two(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
+
+template <class T, bool EDGE>
+__device__ __forceinline__ void store_vec(T* row, int c, int dim, const float2 (&v)[kVec<T> / 2]) {
+  Pack<T> p;
+#pragma unroll
+  for (int t = 0; t < kVec<T> / 2; ++t) pack_two(&p.v[2 * t], v[t]);
+  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
+    *reinterpret_cast<uint4*>(row + c) = p.raw;
+  } else {
+#pragma unroll
+    for (int t = 0; t < kVec<T>; ++t)
+      if ((unsigned)(c + t) < (unsigned)dim) row[c + t] = p.v[t];
+  }
+}
+
+// ---- asynchronous copies -------------------------------------------------------------------------
+// 16 bytes from global to shared memory, the last 16 - bytes of them zero and not read
+__device__ __forceinline__ void copy_async(uint4* to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A thread's own ring of S slots in shared memory for the C vectors of its next rows.  Every thread reads only what it copied
+// itself, so the ring needs no barrier: it is an extension of the registers that keeps (S - 1) C vectors a thread in
+// flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.
+template <class T, int C, int S, bool EDGE>
+struct Ring {
+  uint4* mine;
+  int threads;
+  __device__ __forceinline__ Ring(uint4* smem, int part) : mine(smem + (size_t)part * S * C * blockDim.x + threadIdx.x), threads(blockDim.x) {}
+  // columns [c0 + k advance, + VEC) of `row`; what lies behind the row is zero.  In front of it (c0 < 0) the vector holds what
+  // the 16 bytes hold: the end of the row before, or what precedes the matrix in its allocation; zero_front() clears it.
+  __device__ __forceinline__ void fetch(int slot, const T* row, int c0, int advance, int dim) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = c0 + k * advance, left = (dim - c) * (int)sizeof(T);
+      const int bytes = EDGE ? max(0, min(16, left)) : (left > 0 ? 16 : 0);
+      copy_async(mine + (slot * C + k) * threads, row + (bytes > 0 ? c : c0), bytes);
+    }
+  }
+  __device__ __forceinline__ void read(int slot, Pack<T> (&out)[C], int c0) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) out[k].raw = mine[(slot * C + k) * threads];
+    if (EDGE && c0 < 0) {
+#pragma unroll
+      for (int t = 0; t < kVec<T>; ++t)
+        if (c0 + t < 0) out[0].v[t] = from_float<T>(0.0f);
+    }
+  }
+};
+
+// Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// ---- generator ----------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, uint32_t k0, uint32_t k1) {
+  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    // (the halves of a product one by one: 31 lanes a cycle and SM against 26 for the 64-bit product)
+    const uint32_t ah = __umulhi(0xD2511F53u, c0), al = 0xD2511F53u * c0;
+    const uint32_t bh = __umulhi(0xCD9E8D57u, c2), bl = 0xCD9E8D57u * c2;
+    c0 = bh ^ c1 ^ k0;
+    c2 = ah ^ c3 ^ k1;
+    c1 = bl;
+    c3 = al;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint64_t step_of(const Drop& d) {
+  return d.on && d.step_dev != nullptr ? d.step + (uint64_t)*d.step_dev : d.step;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+__device__ __forceinline__ bool kept(const Drop& d, uint64_t step, int64_t e) {
+  return word(philox7((uint64_t)e >> 2, step, d.k0, d.k1), (int)(e & 3)) > d.last;
+}
+
+// v[k][t] = element e + k advance + t stays ? v[k][t] : 0, N elements for each of C vectors; N and advance are multiples of four.  One
+// Philox call gives the words of four elements that start at a multiple of four.  Elsewhere (EDGE only) the elements lie in
+// N / 4 + 1 such groups; their bits are moved into place first, a path of rows with a stride or an offset of their own.
+// (No branch between the vectors: seven rounds are one long chain of dependent instructions, and only other calls fill it.)
+template <int C, int N, bool EDGE>
+__device__ __forceinline__ void drop_elements(const Drop& d, uint64_t step, int64_t e, int advance, float2 (&v)[C][N / 2]) {
+  const int sh = EDGE ? (int)(e & 3) : 0;
+  if (!EDGE || sh == 0) {
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) {
+        const uint4 w = philox7((uint64_t)((e + k * advance) >> 2) + q, step, d.k0, d.k1);
+        v[k][2 * q].x = w.x > d.last ? v[k][2 * q].x : 0.0f;
+        v[k][2 * q].y = w.y > d.last ? v[k][2 * q].y : 0.0f;
+        v[k][2 * q + 1].x = w.z > d.last ? v[k][2 * q + 1].x : 0.0f;
+        v[k][2 * q + 1].y = w.w > d.last ? v[k][2 * q + 1].y : 0.0f;
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      uint32_t bits = 0;
+      for (int q = 0; q <= N / 4; ++q) {
+        const uint4 w = philox7((uint64_t)((e + k * advance) >> 2) + q, step, d.k0, d.k1);
+        bits |= ((uint32_t)(w.x > d.last) | (uint32_t)(w.y > d.last) << 1 | (uint32_t)(w.z > d.last) << 2 | (uint32_t)(w.w > d.last) << 3) << (4 * q);
+      }
+      bits >>= sh;
+#pragma unroll
+      for (int t = 0; t < N / 2; ++t) v[k][t] = make_float2((bits >> (2 * t)) & 1 ? v[k][t].x : 0.0f, (bits >> (2 * t + 1)) & 1 ? v[k][t].y : 0.0f);
+    }
+  }
+}
+
+// every element times f
+template <int C, int H>
+__device__ __forceinline__ void scale_elements(float2 (&v)[C][H], float f) {
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+#pragma unroll
+    for (int t = 0; t < H; ++t) v[k][t] = __fmul2_rn(v[k][t], both(f));
+}
+
+// relu(z) and its gradient keep a NaN, as torch's do
+__device__ __forceinline__ float relu_of(float z) {
+  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z));
+  return z;
+}
+
+__device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
+
+template <class T>
+__device__ __forceinline__ void unpack(const Pack<T>& p, float2 (&v)[kVec<T> / 2]) {
+#pragma unroll
+  for (int t = 0; t < kVec<T> / 2; ++t) v[t] = make_float2(to_float(p.v[2 * t]), to_float(p.v[2 * t + 1]));
+}
+
+__device__ __forceinline__ float half_of(const float2& v, int i) { return i ? v.y : v.x; }
+
+// ---- groups -------------------------------------------------------------------------------------
+// L = 4..32: lanes of a warp; L = 0: the block is the group
+template <int L>
+struct Group {
+  int lane, lanes, index;      // index: of the group in the block
+  unsigned mask;
+  int64_t first, stride;       // rows of this group: first, first + stride, ...
+  __device__ __forceinline__ Group() {
+    if constexpr (L == 0) {
+      lane = threadIdx.x;
+      lanes = blockDim.x;
+      index = 0;
+      mask = 0xffffffffu;
+      first = blockIdx.x;
+      stride = gridDim.x;
+    } else {
+      lane = threadIdx.x % L;
+      lanes = L;
+      index = threadIdx.x / L;
+      mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << ((threadIdx.x & 31) & ~(L - 1));
+      first = (int64_t)blockIdx.x * (blockDim.x / L) + index;
+      stride = (int64_t)gridDim.x * (blockDim.x / L);
+    }
+  }
+  // Sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
+  // for each of two sums that follow one another (L = 0 only).
+  __device__ __forceinline__ float sum(float v, float* buf) const {
+#pragma unroll
+    for (int o = (L == 0 ? 32 : L) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    if constexpr (L == 0) {
+      const int warps = blockDim.x >> 5;
+      if (warps > 1) {
+        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = (threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)              // at most 16 warps
+          if (o < warps) v += __shfl_xor_sync(mask, v, o);
+        v = __shfl_sync(mask, v, 0);
+      }
+    }
+    return v;
+  }
+  // two sums at once: the first exchange leaves one of them to each half of the group
+  __device__ __forceinline__ float2 sum(float2 v, float* buf) const {
+    constexpr int W = L == 0 ? 32 : L;
+    const bool upper = threadIdx.x & (W / 2);
+    const float other = __shfl_xor_sync(mask, upper ? v.x : v.y, W / 2);
+    float mine = (upper ? v.y : v.x) + other;
+#pragma unroll
+    for (int o = W / 4; o > 0; o >>= 1) mine += __shfl_xor_sync(mask, mine, o);
+    if constexpr (L == 0) {
+      const int warps = blockDim.x >> 5, l = threadIdx.x & 31;
+      if (warps > 1) {
+        if ((threadIdx.x & 15) == 0) buf[(l >> 4) * 16 + (threadIdx.x >> 5)] = mine;
+        __syncthreads();
+        mine = (l & 15) < warps ? buf[l] : 0.0f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+          if (o < warps) mine += __shfl_xor_sync(mask, mine, o);
+      }
+    }
+    return make_float2(__shfl_sync(mask, mine, 0, W), __shfl_sync(mask, mine, W / 2, W));
+  }
+};
+
+}  // namespace
+}  // namespace rof

@@ -11,252 +11,10 @@
 // VEC rows, so a thread's columns never change.  All matrices of a call must share s (EDGE covers it; without
 // EDGE every vector is whole); calls where they do not run on the *_plain kernels.
 #pragma once
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include <algorithm>
-#include <atomic>
-#include <initializer_list>
-
-#include "norm.h"
+#include "norm_device.cuh"
 
 namespace rof {
 namespace {
-
-// ---- types --------------------------------------------------------------------------------------
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-
-template <class T> constexpr int kVec = 16 / (int)sizeof(T);
-
-// a weight or bias vector: 32-bit, or of the matrix's own type
-template <class T>
-__device__ __forceinline__ float vector_at(const void* p, int f32, int i) {
-  return f32 ? __ldg(reinterpret_cast<const float*>(p) + i) : to_float(reinterpret_cast<const T*>(p)[i]);
-}
-
-template <class T>
-__device__ __forceinline__ void vector_put(void* p, int f32, int i, float v) {
-  if (f32) reinterpret_cast<float*>(p)[i] = v;
-  else reinterpret_cast<T*>(p)[i] = from_float<T>(v);
-}
-
-template <class T>
-union Pack {
-  uint4 raw;
-  T v[kVec<T>];
-  __device__ Pack() {}
-};
-
-// columns [c, c + VEC) of a row; what lies outside [0, dim) is zero
-template <class T, bool EDGE>
-__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim) {
-  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
-    out.raw = *reinterpret_cast<const uint4*>(row + c);
-  } else {
-#pragma unroll
-    for (int t = 0; t < kVec<T>; ++t) out.v[t] = (unsigned)(c + t) < (unsigned)dim ? row[c + t] : from_float<T>(0.0f);
-  }
-}
-
-__device__ __forceinline__ void pack_two(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
-__device__ __forceinline__ void pack_two(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
-__device__ __forceinline__ void pack_two(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
-
-template <class T, bool EDGE>
-__device__ __forceinline__ void store_vec(T* row, int c, int dim, const float2 (&v)[kVec<T> / 2]) {
-  Pack<T> p;
-#pragma unroll
-  for (int t = 0; t < kVec<T> / 2; ++t) pack_two(&p.v[2 * t], v[t]);
-  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
-    *reinterpret_cast<uint4*>(row + c) = p.raw;
-  } else {
-#pragma unroll
-    for (int t = 0; t < kVec<T>; ++t)
-      if ((unsigned)(c + t) < (unsigned)dim) row[c + t] = p.v[t];
-  }
-}
-
-// ---- asynchronous copies -------------------------------------------------------------------------
-// 16 bytes from global to shared memory, the last 16 - bytes of them zero and not read
-__device__ __forceinline__ void copy_async(uint4* to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// A thread's own ring of S slots in shared memory for the C vectors of its next rows.  Every thread reads only what it copied
-// itself, so the ring needs no barrier: it is an extension of the registers that keeps (S - 1) C vectors a thread in
-// flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.
-template <class T, int C, int S, bool EDGE>
-struct Ring {
-  uint4* mine;
-  int threads;
-  __device__ __forceinline__ Ring(uint4* smem, int part) : mine(smem + (size_t)part * S * C * blockDim.x + threadIdx.x), threads(blockDim.x) {}
-  // columns [c0 + k advance, + VEC) of `row`; what lies behind the row is zero.  In front of it (c0 < 0) the vector holds what
-  // the 16 bytes hold: the end of the row before, or what precedes the matrix in its allocation; zero_front() clears it.
-  __device__ __forceinline__ void fetch(int slot, const T* row, int c0, int advance, int dim) const {
-#pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance, left = (dim - c) * (int)sizeof(T);
-      const int bytes = EDGE ? max(0, min(16, left)) : (left > 0 ? 16 : 0);
-      copy_async(mine + (slot * C + k) * threads, row + (bytes > 0 ? c : c0), bytes);
-    }
-  }
-  __device__ __forceinline__ void read(int slot, Pack<T> (&out)[C], int c0) const {
-#pragma unroll
-    for (int k = 0; k < C; ++k) out[k].raw = mine[(slot * C + k) * threads];
-    if (EDGE && c0 < 0) {
-#pragma unroll
-      for (int t = 0; t < kVec<T>; ++t)
-        if (c0 + t < 0) out[0].v[t] = from_float<T>(0.0f);
-    }
-  }
-};
-
-// ---- generator ----------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, uint32_t k0, uint32_t k1) {
-  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
-#pragma unroll
-  for (int r = 0; r < 7; ++r) {
-    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
-    c1 = (uint32_t)b;
-    c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return make_uint4(c0, c1, c2, c3);
-}
-
-__device__ __forceinline__ uint64_t step_of(const Drop& d) {
-  return d.on && d.step_dev != nullptr ? d.step + (uint64_t)*d.step_dev : d.step;
-}
-
-__device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-
-__device__ __forceinline__ bool kept(const Drop& d, uint64_t step, int64_t e) {
-  return word(philox7((uint64_t)e >> 2, step, d.k0, d.k1), (int)(e & 3)) > d.last;
-}
-
-// v[t] = element e + t stays ? v[t] : 0 for N elements, N a multiple of 4.  One Philox call gives the words of four elements that
-// start at a multiple of four.  Elsewhere (EDGE only) the elements lie in N / 4 + 1 such groups; their words are moved into
-// place first, a path of rows with a stride or an offset of their own.
-template <int N, bool EDGE>
-__device__ __forceinline__ void drop_elements(const Drop& d, uint64_t step, int64_t e, float2 (&v)[N / 2]) {
-  const int sh = EDGE ? (int)(e & 3) : 0;
-  if (!EDGE || sh == 0) {
-#pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
-      const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
-      v[2 * q].x = w.x > d.last ? v[2 * q].x : 0.0f;
-      v[2 * q].y = w.y > d.last ? v[2 * q].y : 0.0f;
-      v[2 * q + 1].x = w.z > d.last ? v[2 * q + 1].x : 0.0f;
-      v[2 * q + 1].y = w.w > d.last ? v[2 * q + 1].y : 0.0f;
-    }
-  } else {
-    uint32_t bits = 0;
-    for (int q = 0; q <= N / 4; ++q) {
-      const uint4 w = philox7((uint64_t)(e >> 2) + q, step, d.k0, d.k1);
-      bits |= ((uint32_t)(w.x > d.last) | (uint32_t)(w.y > d.last) << 1 | (uint32_t)(w.z > d.last) << 2 | (uint32_t)(w.w > d.last) << 3) << (4 * q);
-    }
-    bits >>= sh;
-#pragma unroll
-    for (int t = 0; t < N / 2; ++t) v[t] = make_float2((bits >> (2 * t)) & 1 ? v[t].x : 0.0f, (bits >> (2 * t + 1)) & 1 ? v[t].y : 0.0f);
-  }
-}
-
-// relu(z) and its gradient keep a NaN, as torch's do
-__device__ __forceinline__ float relu_of(float z) {
-  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z));
-  return z;
-}
-
-__device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
-
-// Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
-template <class T>
-__device__ __forceinline__ void unpack(const Pack<T>& p, float2 (&v)[kVec<T> / 2]) {
-#pragma unroll
-  for (int t = 0; t < kVec<T> / 2; ++t) v[t] = make_float2(to_float(p.v[2 * t]), to_float(p.v[2 * t + 1]));
-}
-
-__device__ __forceinline__ float half_of(const float2& v, int i) { return i ? v.y : v.x; }
-
-// ---- groups -------------------------------------------------------------------------------------
-// L = 4..32: lanes of a warp; L = 0: the block is the group
-template <int L>
-struct Group {
-  int lane, lanes, index;      // index: of the group in the block
-  unsigned mask;
-  int64_t first, stride;       // rows of this group: first, first + stride, ...
-  __device__ __forceinline__ Group() {
-    if constexpr (L == 0) {
-      lane = threadIdx.x;
-      lanes = blockDim.x;
-      index = 0;
-      mask = 0xffffffffu;
-      first = blockIdx.x;
-      stride = gridDim.x;
-    } else {
-      lane = threadIdx.x % L;
-      lanes = L;
-      index = threadIdx.x / L;
-      mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << ((threadIdx.x & 31) & ~(L - 1));
-      first = (int64_t)blockIdx.x * (blockDim.x / L) + index;
-      stride = (int64_t)gridDim.x * (blockDim.x / L);
-    }
-  }
-  // Sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
-  // for each of two sums that follow one another (L = 0 only).
-  __device__ __forceinline__ float sum(float v, float* buf) const {
-#pragma unroll
-    for (int o = (L == 0 ? 32 : L) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-    if constexpr (L == 0) {
-      const int warps = blockDim.x >> 5;
-      if (warps > 1) {
-        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = (threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : 0.0f;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1)              // at most 16 warps
-          if (o < warps) v += __shfl_xor_sync(mask, v, o);
-        v = __shfl_sync(mask, v, 0);
-      }
-    }
-    return v;
-  }
-  // two sums at once: the first exchange leaves one of them to each half of the group
-  __device__ __forceinline__ float2 sum(float2 v, float* buf) const {
-    constexpr int W = L == 0 ? 32 : L;
-    const bool upper = threadIdx.x & (W / 2);
-    const float other = __shfl_xor_sync(mask, upper ? v.x : v.y, W / 2);
-    float mine = (upper ? v.y : v.x) + other;
-#pragma unroll
-    for (int o = W / 4; o > 0; o >>= 1) mine += __shfl_xor_sync(mask, mine, o);
-    if constexpr (L == 0) {
-      const int warps = blockDim.x >> 5, l = threadIdx.x & 31;
-      if (warps > 1) {
-        if ((threadIdx.x & 15) == 0) buf[(l >> 4) * 16 + (threadIdx.x >> 5)] = mine;
-        __syncthreads();
-        mine = (l & 15) < warps ? buf[l] : 0.0f;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1)
-          if (o < warps) mine += __shfl_xor_sync(mask, mine, o);
-      }
-    }
-    return make_float2(__shfl_sync(mask, mine, 0, W), __shfl_sync(mask, mine, W / 2, W));
-  }
-};
 
 // distance of row r's first element from the 16-byte boundary below it
 template <class T, bool EDGE>
@@ -359,27 +117,26 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
     minus = both(-mean);
     const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
     if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int t = 0; t < H; ++t) v[k][t] = __ffma2_rn(__fmul2_rn(__fadd2_rn(v[k][t], minus), both(rstd)), w[k][t], b[k][t]);
+    if constexpr (HIDDEN) {
+      if (a.relu) {
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int t = 0; t < H; ++t) v[k][t] = make_float2(relu_of(v[k][t].x), relu_of(v[k][t].y));
+      }
+      if (a.drop.on) {
+        scale_elements(v, a.drop.scale);
+        drop_elements<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, v);
+      }
+    }
     T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance;
-      if (c >= a.dim) continue;
-      float2 o[H];
-#pragma unroll
-      for (int t = 0; t < H; ++t) o[t] = __ffma2_rn(__fmul2_rn(__fadd2_rn(v[k][t], minus), both(rstd)), w[k][t], b[k][t]);
-      if constexpr (HIDDEN) {
-        if (a.relu) {
-#pragma unroll
-          for (int t = 0; t < H; ++t) o[t] = make_float2(relu_of(o[t].x), relu_of(o[t].y));
-        }
-        if (a.drop.on) {
-#pragma unroll
-          for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(o[t], both(a.drop.scale));
-          drop_elements<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c, o);
-        }
-      }
-      store_vec<T, EDGE>(y, c, a.dim, o);
-    }
+    for (int k = 0; k < C; ++k)
+      if (c0 + k * advance < a.dim) store_vec<T, EDGE>(y, c0 + k * advance, a.dim, v[k]);
   }
 }
 
@@ -468,17 +225,16 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
     const float2 minus = both(-st.x), rstd = both(st.y);
     float2 h[C][H], gr[C][H], s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance;
-      unpack<T>(rx[k], h[k]);
-      unpack<T>(rd[k], gr[k]);
-      if constexpr (HIDDEN) {
-        if (a.drop.on && c < a.dim) {
-#pragma unroll
-          for (int t = 0; t < H; ++t) gr[k][t] = __fmul2_rn(gr[k][t], both(a.drop.scale));
-          drop_elements<V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c, gr[k]);
-        }
+    for (int k = 0; k < C; ++k) unpack<T>(rd[k], gr[k]);
+    if constexpr (HIDDEN) {
+      if (a.drop.on) {
+        scale_elements(gr, a.drop.scale);
+        drop_elements<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, gr);
       }
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      unpack<T>(rx[k], h[k]);
 #pragma unroll
       for (int t = 0; t < H; ++t) {
         // (a column outside the row has x = dy = 0 and adds nothing anywhere)
@@ -633,68 +389,74 @@ __global__ void __launch_bounds__(128) norm_backward_columns_plain(const __grid_
 }
 
 // ---- dropout ------------------------------------------------------------------------------------
-// one vector: BACK = false: drop(relu?(x + b)); BACK = true: dy behind the dropout and the ReLU, where with the ReLU
-// the forward's output y says which elements were kept and positive
-template <class T, bool BACK, bool EDGE>
-__device__ __forceinline__ void drop_vec(const DropArgs& a, uint64_t step, int64_t e, const Pack<T>& in, const Pack<T>& y,
-                                         const float2 (&b)[kVec<T> / 2], float2 (&o)[kVec<T> / 2]) {
+// U vectors that lie `advance` elements apart, e the index of the first.  BACK = false: drop(relu?(x + b)); BACK = true: dy behind the
+// dropout and the ReLU, where with the ReLU the forward's output y says which elements were kept and positive.  DRAW: the
+// generator is asked.
+template <class T, int U, bool BACK, bool DRAW, bool EDGE>
+__device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, int64_t e, int64_t advance, const Pack<T> (&in)[U],
+                                             const Pack<T> (&y)[U], const float2 (&b)[kVec<T> / 2], float2 (&o)[U][kVec<T> / 2]) {
   constexpr int V = kVec<T>, H = V / 2;
-  unpack<T>(in, o);
-  if constexpr (BACK) {
-    if (a.relu) {
-      float2 f[H];
-      unpack<T>(y, f);
 #pragma unroll
-      for (int t = 0; t < H; ++t) o[t] = make_float2(f[t].x <= 0.0f ? 0.0f : o[t].x, f[t].y <= 0.0f ? 0.0f : o[t].y);
-    }
-  } else {
+  for (int u = 0; u < U; ++u) {
+    unpack<T>(in[u], o[u]);
+    if constexpr (BACK) {
+      if (!DRAW && a.relu) {
+        float2 f[H];
+        unpack<T>(y[u], f);
 #pragma unroll
-    for (int t = 0; t < H; ++t) o[t] = __fadd2_rn(o[t], b[t]);
-    if (a.relu) {
+        for (int t = 0; t < H; ++t) o[u][t] = make_float2(f[t].x <= 0.0f ? 0.0f : o[u][t].x, f[t].y <= 0.0f ? 0.0f : o[u][t].y);
+      }
+    } else {
 #pragma unroll
-      for (int t = 0; t < H; ++t) o[t] = make_float2(relu_of(o[t].x), relu_of(o[t].y));
+      for (int t = 0; t < H; ++t) o[u][t] = __fadd2_rn(o[u][t], b[t]);
+      if (a.relu) {
+#pragma unroll
+        for (int t = 0; t < H; ++t) o[u][t] = make_float2(relu_of(o[u][t].x), relu_of(o[u][t].y));
+      }
     }
   }
-  if (a.drop.on) {
+  scale_elements(o, a.drop.scale);
+  if constexpr (DRAW) {
 #pragma unroll
-    for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(o[t], both(a.drop.scale));
-    if (!(BACK && a.relu)) drop_elements<V, EDGE>(a.drop, step, e, o);
+    for (int u = 0; u < U; ++u) {
+      float2 (&one)[1][H] = *reinterpret_cast<float2(*)[1][H]>(&o[u]);
+      drop_elements<1, V, EDGE>(a.drop, step, e + u * advance, 0, one);
+    }
   }
 }
 
-// contiguous matrices without a bias: one run of n elements from an aligned address
-template <class T, bool BACK, bool EDGE>
-__global__ void __launch_bounds__(256) dropout_flat_kernel(const __grid_constant__ DropArgs a, int64_t n) {
-  constexpr int V = kVec<T>, U = 2;
-  const uint64_t step = step_of(a.drop);
+// Contiguous matrices without a bias: one run of n elements from an aligned address.  A block takes U x 256 vectors side by side and
+// is done: U = 4 vectors a thread (2 where two matrices are read) are enough calls to fill the generator's chains.  Bound by HBM in 32 bits
+// and, with the generator, almost by instructions in 16.
+template <class T, bool BACK, bool DRAW, bool EDGE>
+__global__ void __launch_bounds__(256, 4) dropout_flat_kernel(const __grid_constant__ DropArgs a, int64_t n) {
+  constexpr int V = kVec<T>, U = BACK && !DRAW ? 2 : 4;
+  const uint64_t step = DRAW ? step_of(a.drop) : 0;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* y = reinterpret_cast<const T*>(a.y);
   T* out = reinterpret_cast<T*>(a.out);
-  const bool two = BACK && a.relu;
+  const bool two = BACK && !DRAW && a.relu;
   const float2 zero[V / 2] = {};
-  const int64_t vectors = n / V, stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vectors; i += U * stride) {
-    Pack<T> in[U], yy[U];
+  const int64_t vectors = n / V, i = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  Pack<T> in[U], yy[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * stride < vectors) {
-        in[u].raw = reinterpret_cast<const uint4*>(x)[i + u * stride];
-        if (two) yy[u].raw = reinterpret_cast<const uint4*>(y)[i + u * stride];
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * stride < vectors) {
-        float2 o[V / 2];
-        const int64_t e = (i + u * stride) * V;
-        drop_vec<T, BACK, EDGE>(a, step, a.drop.first + e, in[u], yy[u], zero, o);
-        store_vec<T, false>(out + e, 0, V, o);
-      }
+  for (int u = 0; u < U; ++u) {
+    in[u].raw = yy[u].raw = make_uint4(0, 0, 0, 0);
+    if (i + u * 256 < vectors) {
+      in[u].raw = reinterpret_cast<const uint4*>(x)[i + u * 256];
+      if (two) yy[u].raw = reinterpret_cast<const uint4*>(y)[i + u * 256];
+    }
   }
+  float2 o[U][V / 2];
+  drop_vectors<T, U, BACK, DRAW, EDGE>(a, step, a.drop.first + i * V, 256 * V, in, yy, zero, o);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (i + u * 256 < vectors) store_vec<T, false>(out + (i + u * 256) * V, 0, V, o[u]);
   // the last elements that fill no vector
   const int64_t e = vectors * V + threadIdx.x;
   if (blockIdx.x == 0 && e < n) {
     float z = to_float(x[e]);
-    const bool keep = !a.drop.on || two || kept(a.drop, step, a.drop.first + e);
+    const bool keep = !DRAW || kept(a.drop, step, a.drop.first + e);
     if (!BACK && a.relu) z = relu_of(z);
     if (two && to_float(y[e]) <= 0.0f) z = 0.0f;
     out[e] = from_float<T>(keep ? z * a.drop.scale : 0.0f);
@@ -702,7 +464,7 @@ __global__ void __launch_bounds__(256) dropout_flat_kernel(const __grid_constant
 }
 
 // thread = vector `col` of the rows row0, row0 + stride, ...; a.lanes threads side by side cover a tile of a row
-template <class T, bool BACK, bool EDGE>
+template <class T, bool BACK, bool DRAW, bool EDGE>
 __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
   constexpr int V = kVec<T>, U = 4;
   extern __shared__ float columns[];
@@ -711,8 +473,8 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
   const int s = row_shift<T, EDGE>(a.x, a.ldx, first);
   const int c = (int)(blockIdx.y * a.lanes + lane) * V - s;
   const bool live = group < groups && c < a.dim;
-  const uint64_t step = step_of(a.drop);
-  const bool two = BACK && a.relu;
+  const uint64_t step = DRAW ? step_of(a.drop) : 0;
+  const bool two = BACK && !DRAW && a.relu;
   float2 b[1][V / 2], acc[V / 2];
   load_columns<T, 1>(b, !BACK && live ? a.bias : nullptr, a.bf32, a.dim, c, 0, 0.0f);
 #pragma unroll
@@ -721,21 +483,23 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
     for (int64_t r = first; r < a.rows; r += U * stride) {
       Pack<T> in[U], yy[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        in[u].raw = yy[u].raw = make_uint4(0, 0, 0, 0);
         if (r + u * stride < a.rows) {
           load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim);
           if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim);
         }
+      }
+      float2 o[U][V / 2];
+      drop_vectors<T, U, BACK, DRAW, EDGE>(a, step, a.drop.first + r * a.dim + c, stride * a.dim, in, yy, b[0], o);
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + u * stride < a.rows) {
-          float2 o[V / 2];
-          drop_vec<T, BACK, EDGE>(a, step, a.drop.first + (r + u * stride) * a.dim + c, in[u], yy[u], b[0], o);
           if constexpr (BACK) {
 #pragma unroll
-            for (int t = 0; t < V / 2; ++t) acc[t] = __fadd2_rn(acc[t], o[t]);
+            for (int t = 0; t < V / 2; ++t) acc[t] = __fadd2_rn(acc[t], o[u][t]);
           }
-          if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o);
+          if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o[u]);
         }
     }
   }
@@ -987,14 +751,16 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
   if (a.rows <= 1) a.ldx = a.ldy = a.ldo = 0;
   constexpr int V = kVec<T>;
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.y, a.ldy}, {a.out, a.ldo}});
+  const bool draw = a.drop.on && !(BACK && a.relu);
   const auto whole = [&](const void* p, int64_t ld) {
     return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (a.rows == 1 || ld == a.dim));
   };
   if (a.partial == nullptr && a.bias == nullptr && whole(a.x, a.ldx) && whole(a.y, a.ldy) && whole(a.out, a.ldo)) {
     const int64_t n = a.rows * a.dim;
-    const int blocks = clamp_blocks((n / V + 511) / 512, kSMs * 16);
-    if (a.drop.first % 4 == 0) dropout_flat_kernel<T, BACK, false><<<blocks, 256, 0, stream>>>(a, n);
-    else dropout_flat_kernel<T, BACK, true><<<blocks, 256, 0, stream>>>(a, n);
+    const int per = BACK && !draw ? 512 : 1024, blocks = (int)std::max<int64_t>(1, (n / V + per - 1) / per);
+    if (!draw) dropout_flat_kernel<T, BACK, false, false><<<blocks, 256, 0, stream>>>(a, n);
+    else if (a.drop.first % 4 == 0) dropout_flat_kernel<T, BACK, true, false><<<blocks, 256, 0, stream>>>(a, n);
+    else dropout_flat_kernel<T, BACK, true, true><<<blocks, 256, 0, stream>>>(a, n);
     return cudaGetLastError();
   }
   const int tiles = (l.vectors + 255) / 256;
@@ -1007,8 +773,10 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
     blocks = blocks < 8 ? 8 : blocks / 8 * 8;
     const int smem = BACK && a.partial != nullptr ? groups * a.lanes * V * 4 : 0;
     const dim3 grid(blocks, tiles);
-    if (l.edge) dropout_rows_kernel<T, BACK, true><<<grid, threads, smem, stream>>>(a);
-    else dropout_rows_kernel<T, BACK, false><<<grid, threads, smem, stream>>>(a);
+    if (draw && l.edge) dropout_rows_kernel<T, BACK, true, true><<<grid, threads, smem, stream>>>(a);
+    else if (draw) dropout_rows_kernel<T, BACK, true, false><<<grid, threads, smem, stream>>>(a);
+    else if (l.edge) dropout_rows_kernel<T, BACK, false, true><<<grid, threads, smem, stream>>>(a);
+    else dropout_rows_kernel<T, BACK, false, false><<<grid, threads, smem, stream>>>(a);
   } else {
     if (a.out != nullptr) dropout_plain<T, BACK><<<clamp_blocks((a.rows * a.dim + 255) / 256, kSMs * 8), 256, 0, stream>>>(a);
     if (BACK && a.partial != nullptr) {
