@@ -20,7 +20,8 @@ LIB = os.path.join(PKG, "_lib")
 INCLUDE = os.path.join(ROOT, "include")
 
 CUDA_SOURCES = ["plan.cu", "kernels.cu", "api.cu", "stages.cu", "static_scratch.cu", "norm.cu",
-                "norm_f32.cu", "norm_bf16.cu", "norm_f16.cu"]
+                "norm_f32.cu", "norm_bf16.cu", "norm_f16.cu",
+                "norm_tile_f32.cu", "norm_tile_bf16.cu", "norm_tile_f16.cu"]
 HOST_SOURCES = [os.path.join("host", "graphgen.cpp"), os.path.join("host", "reuse_search.cpp")]
 
 NVCC_FLAGS = [

@@ -51,7 +51,8 @@ int check_matrix(const char* who, const char* name, int dtype, const void* p, in
 
 // the kernels' form of a rof_dropout
 int read_drop(const char* who, const rof_dropout* d, int64_t rows, int dim, Drop* out) {
-  *out = Drop{0, 0, 1.0f, 0, 0, 0, nullptr, 0};
+  *out = Drop{};
+  out->scale = 1.0f;
   if (d == nullptr) return ROF_OK;
   if (!(d->p >= 0.0 && d->p <= 1.0)) return bad(who, "p is not in [0, 1]");
   if (d->first_row < 0 || (dim > 0 && d->first_row > INT64_MAX / 8 / dim)) return bad(who, "first_row out of range");
@@ -61,8 +62,10 @@ int read_drop(const char* who, const rof_dropout* d, int64_t rows, int dim, Drop
   out->on = 1;
   out->last = (uint32_t)((uint64_t)border - 1);
   out->scale = d->p < 1.0 ? (float)(1.0 / (1.0 - d->p)) : 0.0f;
-  out->k0 = (uint32_t)d->seed;
-  out->k1 = (uint32_t)(d->seed >> 32);
+  for (int i = 0; i < 7; ++i) {                    // the key moves on by these two constants from round to round
+    out->key[2 * i] = (uint32_t)d->seed + (uint32_t)i * 0x9E3779B9u;
+    out->key[2 * i + 1] = (uint32_t)(d->seed >> 32) + (uint32_t)i * 0xBB67AE85u;
+  }
   out->step = d->step;
   out->step_dev = d->step_dev;
   out->first = d->first_row * dim;

@@ -12,7 +12,7 @@ struct Drop {
   uint32_t on;         // 0: no element is dropped (scale is 1)
   uint32_t last;       // words up to this one are dropped
   float scale;         // 1 / (1 - p)
-  uint32_t k0, k1;     // key
+  uint32_t key[14];    // of the seven rounds: two words each
   uint64_t step;
   const int64_t* step_dev;   // added to `step` when the kernel runs
   int64_t first;       // index of the matrix's first element in the whole one
@@ -52,12 +52,31 @@ inline int column_blocks_cap(int64_t rows, int dim) {
   return (int)std::min<int64_t>(cap, (std::max<int64_t>(rows, 1) + 7) / 8 * 8);
 }
 
+// The tile kernels (norm_tile.cuh).
+enum TileMode { kNormForward, kNormForwardHidden, kNormBackward, kNormBackwardHidden, kDropForward, kDropBackward };
+
+constexpr int kTileMaxColumns = 511;
+
+struct RowRunArgs {
+  const void* a;            // x, or a dropout's dy
+  const void* b;            // a norm's dy, or the dropout's output (null: not read)
+  void* out;
+  const void* weight; const void* bias; int f32;
+  float2* stats;
+  float* partial;           // [blocks][2 (norm) or 1][dim]
+  int64_t rows; int dim;
+  float eps; int relu;
+  Drop drop;
+};
+
 struct NormLaunchers {
   cudaError_t (*norm_forward)(const NormArgs&, cudaStream_t);
   cudaError_t (*norm_backward)(const NormArgs&, cudaStream_t);
   cudaError_t (*dropout_forward)(const DropArgs&, cudaStream_t);
   cudaError_t (*dropout_backward)(const DropArgs&, cudaStream_t);
 };
+using TileLauncher = cudaError_t (*)(const RowRunArgs&, int mode, cudaStream_t, int* blocks);
+extern const TileLauncher tile_launcher_f32, tile_launcher_bf16, tile_launcher_f16;
 extern const NormLaunchers norm_launchers_f32, norm_launchers_bf16, norm_launchers_f16;
 
 }  // namespace rof

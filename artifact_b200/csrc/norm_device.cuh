@@ -114,19 +114,17 @@ struct Ring {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // ---- generator ----------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, uint32_t k0, uint32_t k1) {
+__device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, const uint32_t (&key)[14]) {
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
     // (the halves of a product one by one: 31 lanes a cycle and SM against 26 for the 64-bit product)
     const uint32_t ah = __umulhi(0xD2511F53u, c0), al = 0xD2511F53u * c0;
     const uint32_t bh = __umulhi(0xCD9E8D57u, c2), bl = 0xCD9E8D57u * c2;
-    c0 = bh ^ c1 ^ k0;
-    c2 = ah ^ c3 ^ k1;
+    c0 = bh ^ c1 ^ key[2 * r];
+    c2 = ah ^ c3 ^ key[2 * r + 1];
     c1 = bl;
     c3 = al;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -138,40 +136,46 @@ __device__ __forceinline__ uint64_t step_of(const Drop& d) {
 __device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
 __device__ __forceinline__ bool kept(const Drop& d, uint64_t step, int64_t e) {
-  return word(philox7((uint64_t)e >> 2, step, d.k0, d.k1), (int)(e & 3)) > d.last;
+  return word(philox7((uint64_t)e >> 2, step, d.key), (int)(e & 3)) > d.last;
 }
 
-// v[k][t] = element e + k advance + t stays ? v[k][t] : 0, N elements for each of C vectors; N and advance are multiples of four.  One
-// Philox call gives the words of four elements that start at a multiple of four.  Elsewhere (EDGE only) the elements lie in
-// N / 4 + 1 such groups; their bits are moved into place first, a path of rows with a stride or an offset of their own.
-// (No branch between the vectors: seven rounds are one long chain of dependent instructions, and only other calls fill it.)
+// The words of C runs of N elements: w[k N + t] is that of element e + k advance + t; N and advance are multiples of four.  One
+// Philox call gives the words of four elements that start at a multiple of four.  Elsewhere (EDGE only: rows with a stride or an
+// offset of their own) the elements lie in N / 4 + 1 such groups.  (No branch between the calls: seven rounds are one long
+// chain of dependent instructions, and only other calls fill it.)
 template <int C, int N, bool EDGE>
-__device__ __forceinline__ void drop_elements(const Drop& d, uint64_t step, int64_t e, int advance, float2 (&v)[C][N / 2]) {
+__device__ __forceinline__ void draw_words(const Drop& d, uint64_t step, int64_t e, int advance, uint32_t (&w)[C * N]) {
   const int sh = EDGE ? (int)(e & 3) : 0;
   if (!EDGE || sh == 0) {
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-#pragma unroll
-      for (int q = 0; q < N / 4; ++q) {
-        const uint4 w = philox7((uint64_t)((e + k * advance) >> 2) + q, step, d.k0, d.k1);
-        v[k][2 * q].x = w.x > d.last ? v[k][2 * q].x : 0.0f;
-        v[k][2 * q].y = w.y > d.last ? v[k][2 * q].y : 0.0f;
-        v[k][2 * q + 1].x = w.z > d.last ? v[k][2 * q + 1].x : 0.0f;
-        v[k][2 * q + 1].y = w.w > d.last ? v[k][2 * q + 1].y : 0.0f;
-      }
+    for (int i = 0; i < C * N / 4; ++i) {
+      const uint4 g = philox7((uint64_t)((e + i / (N / 4) * advance) >> 2) + i % (N / 4), step, d.key);
+      w[4 * i] = g.x;
+      w[4 * i + 1] = g.y;
+      w[4 * i + 2] = g.z;
+      w[4 * i + 3] = g.w;
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      uint32_t bits = 0;
-      for (int q = 0; q <= N / 4; ++q) {
-        const uint4 w = philox7((uint64_t)((e + k * advance) >> 2) + q, step, d.k0, d.k1);
-        bits |= ((uint32_t)(w.x > d.last) | (uint32_t)(w.y > d.last) << 1 | (uint32_t)(w.z > d.last) << 2 | (uint32_t)(w.w > d.last) << 3) << (4 * q);
-      }
-      bits >>= sh;
+      uint4 a = philox7((uint64_t)((e + k * advance) >> 2), step, d.key);
 #pragma unroll
-      for (int t = 0; t < N / 2; ++t) v[k][t] = make_float2((bits >> (2 * t)) & 1 ? v[k][t].x : 0.0f, (bits >> (2 * t + 1)) & 1 ? v[k][t].y : 0.0f);
+      for (int q = 0; q < N / 4; ++q) {
+        const uint4 b = philox7((uint64_t)((e + k * advance) >> 2) + q + 1, step, d.key);
+        uint32_t* o = &w[k * N + 4 * q];
+        o[0] = sh == 1 ? a.y : sh == 2 ? a.z : a.w;
+        o[1] = sh == 1 ? a.z : sh == 2 ? a.w : b.x;
+        o[2] = sh == 1 ? a.w : sh == 2 ? b.x : b.y;
+        o[3] = sh == 1 ? b.x : sh == 2 ? b.y : b.z;
+        a = b;
+      }
     }
   }
+}
+
+// what stays of two elements with the words w[0] and w[1]
+__device__ __forceinline__ float2 kept_of(const Drop& d, const uint32_t* w, float2 v) {
+  return make_float2(w[0] > d.last ? v.x : 0.0f, w[1] > d.last ? v.y : 0.0f);
 }
 
 // every element times f
@@ -264,6 +268,28 @@ struct Group {
     return make_float2(__shfl_sync(mask, mine, 0, W), __shfl_sync(mask, mine, W / 2, W));
   }
 };
+
+// ---- launches -----------------------------------------------------------------------------------
+constexpr int kSMs = 148;
+
+// Lets a kernel have `smem` bytes of dynamic shared memory (and its static ones: 48 KB together need no leave) on the current
+// device; `done`: a bit per device that was seen.
+template <class K>
+void allow_smem(K kernel, int smem, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (smem <= 46 << 10 || cudaGetDevice(&device) != cudaSuccess) return;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+template <class K>
+int blocks_per_sm(K kernel, int threads, int smem) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
+}
+
+inline int clamp_blocks(int64_t wanted, int64_t most) { return (int)std::max<int64_t>(1, std::min(wanted, most)); }
 
 }  // namespace
 }  // namespace rof

@@ -24,10 +24,10 @@ __device__ __forceinline__ int row_shift(const void* base, int64_t ld, int64_t r
 }
 
 // Blocks of 256 threads per SM that the register allocation aims at: as many as leave nothing spilled.
-template <class T, int C, bool HIDDEN>
-constexpr int forward_blocks() { return C * kVec<T> <= 8 ? 4 : C * kVec<T> <= (HIDDEN ? 12 : 16) ? 3 : 2; }
-template <class T, int C, bool HIDDEN>
-constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? 2 : 1; }
+template <class T, int C, bool HIDDEN, bool EDGE>
+constexpr int forward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN && EDGE ? 3 : 4) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? (HIDDEN && EDGE ? 2 : 3) : HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : 2; }
+template <class T, int C, bool HIDDEN, bool EDGE>
+constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 8 : 16) ? 2 : 1; }
 // Slots of the rings
 template <int C>
 constexpr int ring_slots() { return C == 1 ? 4 : C <= 4 ? 3 : 2; }
@@ -52,7 +52,7 @@ __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v))
 
 // HIDDEN: with the ReLU or the dropout (or both)
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN, EDGE>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
@@ -129,8 +129,13 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
           for (int t = 0; t < H; ++t) v[k][t] = make_float2(relu_of(v[k][t].x), relu_of(v[k][t].y));
       }
       if (a.drop.on) {
+        uint32_t words[C * V];
+        draw_words<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, words);
         scale_elements(v, a.drop.scale);
-        drop_elements<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, v);
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int t = 0; t < H; ++t) v[k][t] = kept_of(a.drop, words + k * V + 2 * t, v[k][t]);
       }
     }
     T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
@@ -175,7 +180,7 @@ __device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2
 
 // dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, EDGE>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
@@ -211,6 +216,10 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
     if constexpr (EDGE) not_hoisted(c0);
     const float2 st = st_next;
     if (r + g.stride < a.rows) st_next = a.stats[r + g.stride];
+    uint32_t words[HIDDEN ? C * V : 1];             // drawn while the row is on its way
+    if constexpr (HIDDEN) {
+      if (a.drop.on) draw_words<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, words);
+    }
     Pack<T> rx[C], rd[C];
     copy_wait<S - 2>();
     ring_x.read(slot, rx, c0);
@@ -229,7 +238,10 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
     if constexpr (HIDDEN) {
       if (a.drop.on) {
         scale_elements(gr, a.drop.scale);
-        drop_elements<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, gr);
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+          for (int t = 0; t < H; ++t) gr[k][t] = kept_of(a.drop, words + k * V + 2 * t, gr[k][t]);
       }
     }
 #pragma unroll
@@ -419,8 +431,10 @@ __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, i
   if constexpr (DRAW) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float2 (&one)[1][H] = *reinterpret_cast<float2(*)[1][H]>(&o[u]);
-      drop_elements<1, V, EDGE>(a.drop, step, e + u * advance, 0, one);
+      uint32_t words[V];
+      draw_words<1, V, EDGE>(a.drop, step, e + u * advance, 0, words);
+#pragma unroll
+      for (int t = 0; t < H; ++t) o[u][t] = kept_of(a.drop, words + 2 * t, o[u][t]);
     }
   }
 }
@@ -564,8 +578,6 @@ __global__ void __launch_bounds__(128) dropout_columns_plain(const __grid_consta
 }
 
 // ---- launches -----------------------------------------------------------------------------------
-constexpr int kSMs = 148;
-
 // How the rows of a call's matrices lie against the 16-byte boundaries.  vec: the same way in all of them; edge: there are
 // partial vectors; vectors: of a row, at most.
 struct Layout {
@@ -597,25 +609,6 @@ Layout layout_of(int64_t rows, int dim, std::initializer_list<Matrix> all) {
   return {true, dim % V != 0 || shift != 0, (int)(((int64_t)dim + shift + V - 1) / V)};
 }
 
-// Lets a kernel have `smem` bytes of dynamic shared memory (and its static ones: 48 KB together need no leave) on the current
-// device; `done`: a bit per device that was seen.
-template <class K>
-void allow_smem(K kernel, int smem, std::atomic<uint64_t>& done) {
-  int device = 0;
-  if (smem <= 46 << 10 || cudaGetDevice(&device) != cudaSuccess) return;
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (done.load(std::memory_order_relaxed) & bit) return;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-}
-
-template <class K>
-int blocks_per_sm(K kernel, int threads, int smem) {
-  int n = 0;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
-}
-
-inline int clamp_blocks(int64_t wanted, int64_t most) { return (int)std::max<int64_t>(1, std::min(wanted, most)); }
-
 // a block per row
 template <int C, class F>
 bool wide_rows(int vectors, F&& f) {
@@ -627,9 +620,28 @@ bool wide_rows(int vectors, F&& f) {
 
 // Group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads).  The
 // fewest lanes whose registers hold the row: they have the most bytes in flight each and the fewest steps in the row's sums.
-template <class T, class F>
+// MANY: the backward pass through a ReLU or a dropout also keeps the biases, and gets by with fewer elements a thread.
+template <class T, bool MANY, class F>
 bool by_width(int vectors, F&& f) {
-  if constexpr (sizeof(T) == 4) {                // up to 20 elements per thread
+  if constexpr (MANY && sizeof(T) == 4) {
+    if (vectors <= 4) f.template operator()<4, 1>(256);
+    else if (vectors <= 8) f.template operator()<4, 2>(256);
+    else if (vectors <= 16) f.template operator()<8, 2>(256);
+    else if (vectors <= 24) f.template operator()<8, 3>(256);
+    else if (vectors <= 32) f.template operator()<16, 2>(256);
+    else if (vectors <= 48) f.template operator()<16, 3>(256);
+    else if (vectors <= 64) f.template operator()<32, 2>(256);
+    else if (vectors <= 96) f.template operator()<32, 3>(256);
+    else if (vectors <= 128) f.template operator()<32, 4>(256);
+    else return wide_rows<4>(vectors, f);
+  } else if constexpr (MANY) {
+    if (vectors <= 4) f.template operator()<4, 1>(256);
+    else if (vectors <= 8) f.template operator()<8, 1>(256);
+    else if (vectors <= 16) f.template operator()<16, 1>(256);
+    else if (vectors <= 32) f.template operator()<32, 1>(256);
+    else if (vectors <= 64) f.template operator()<32, 2>(256);
+    else return wide_rows<2>(vectors, f);
+  } else if constexpr (sizeof(T) == 4) {                // up to 20 elements per thread
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<4, 2>(256);
     else if (vectors <= 12) f.template operator()<4, 3>(256);
@@ -699,6 +711,19 @@ struct NormBackward {
   }
 };
 
+// whether the tile kernels take the call: contiguous matrices from 16-byte boundaries, rows that are not whole vectors
+template <class T>
+bool tiled(int64_t rows, int dim, std::initializer_list<Matrix> all) {
+  if (dim > kTileMaxColumns || dim % kVec<T> == 0) return false;
+  for (const Matrix& m : all)
+    if (m.p != nullptr && ((reinterpret_cast<uintptr_t>(m.p) & 15) != 0 || (rows > 1 && m.ld != dim))) return false;
+  return true;
+}
+
+inline TileLauncher tile_launcher(float) { return tile_launcher_f32; }
+inline TileLauncher tile_launcher(__nv_bfloat16) { return tile_launcher_bf16; }
+inline TileLauncher tile_launcher(__half) { return tile_launcher_f16; }
+
 template <class T>
 cudaError_t launch_join(const float* partial, int blocks, int width, int split, void* first, void* second, int f32, cudaStream_t stream) {
   join_columns_kernel<T><<<(width + 31) / 32, 256, 0, stream>>>(partial, blocks, width, split, first, second, f32);
@@ -714,11 +739,15 @@ inline NormArgs one_row(NormArgs a) {
 template <class T>
 cudaError_t launch_norm_forward(const NormArgs& given, cudaStream_t stream) {
   const NormArgs a = one_row(given);
+  if (tiled<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}})) {
+    const RowRunArgs t{a.x, nullptr, a.out, a.weight, a.bias, a.wf32, a.stats, nullptr, a.rows, a.dim, a.eps, a.relu, a.drop};
+    return tile_launcher(T{})(t, a.relu || a.drop.on ? kNormForwardHidden : kNormForward, stream, nullptr);
+  }
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
   bool done = false;
   if (l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, true, false>{a, stream});
-    else done = l.edge ? by_width<T>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T>(l.vectors, NormForward<T, false, false>{a, stream});
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T, false>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T, false>(l.vectors, NormForward<T, true, false>{a, stream});
+    else done = l.edge ? by_width<T, false>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T, false>(l.vectors, NormForward<T, false, false>{a, stream});
   }
   if (!done) norm_forward_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
   return cudaGetLastError();
@@ -728,11 +757,16 @@ template <class T>
 cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
   const NormArgs a = one_row(given);
   int blocks = 0;
+  bool done = tiled<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
+  if (done) {
+    const RowRunArgs t{a.x, a.dy, a.out, a.weight, a.bias, a.wf32, a.stats, a.partial, a.rows, a.dim, a.eps, a.relu, a.drop};
+    const cudaError_t e = tile_launcher(T{})(t, a.relu || a.drop.on ? kNormBackwardHidden : kNormBackward, stream, &blocks);
+    if (e != cudaSuccess) return e;
+  }
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
-  bool done = false;
-  if (l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
-    else done = l.edge ? by_width<T>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
+  if (!done && l.vec) {
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T, true>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T, true>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
+    else done = l.edge ? by_width<T, false>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T, false>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
   }
   if (!done) {
     if (a.out != nullptr) norm_backward_rows_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
@@ -765,7 +799,11 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
   }
   const int tiles = (l.vectors + 255) / 256;
   int blocks = 0;
-  if (l.vec && tiles <= 65535) {
+  if (tiled<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.y, a.ldy}, {a.out, a.ldo}})) {
+    const RowRunArgs t{a.x, a.y, a.out, nullptr, a.bias, a.bf32, nullptr, a.partial, a.rows, a.dim, 0.0f, a.relu, a.drop};
+    const cudaError_t e = tile_launcher(T{})(t, BACK ? kDropBackward : kDropForward, stream, &blocks);
+    if (e != cudaSuccess) return e;
+  } else if (l.vec && tiles <= 65535) {
     a.lanes = std::min(l.vectors, 256);
     const int groups = 256 / a.lanes, threads = (groups * a.lanes + 31) / 32 * 32;
     const int64_t most = a.partial != nullptr ? column_blocks_cap(a.rows, a.dim) : kMaxColumnBlocks;
