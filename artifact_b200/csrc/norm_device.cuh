@@ -83,32 +83,56 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 
 // A thread's own ring of S slots in shared memory for the C vectors of its next rows.  Every thread reads only what it copied
 // itself, so the ring needs no barrier: it is an extension of the registers that keeps (S - 1) C vectors a thread in
-// flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.
-template <class T, int C, int S, bool EDGE>
+// flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.  Vectors that lie behind the
+// row are cleared once and never copied.
+//
+// The kernels are short of instruction slots as much as of bandwidth in 16 bits, so addresses run along: `from` points to column c0 of the
+// next row to fetch, and only additions remain in the loop.
+template <class T, int L, int C, int S, bool EDGE>
 struct Ring {
-  uint4* mine;
-  int threads;
-  __device__ __forceinline__ Ring(uint4* smem, int part) : mine(smem + (size_t)part * S * C * blockDim.x + threadIdx.x), threads(blockDim.x) {}
-  // columns [c0 + k advance, + VEC) of `row`; what lies behind the row is zero.  In front of it (c0 < 0) the vector holds what
-  // the 16 bytes hold: the end of the row before, or what precedes the matrix in its allocation; zero_front() clears it.
-  __device__ __forceinline__ void fetch(int slot, const T* row, int c0, int advance, int dim) const {
+  char* mine;                // this thread's first vector of slot 0
+  const char* from;
+  int64_t row_bytes;         // from one row of the group to its next
+  int left, advance;         // bytes from c0 to the end of the row; between two of the thread's vectors
+  int threads;               // of the block
+  __device__ __forceinline__ Ring(uint4* smem, int part, const void* base, int64_t ld, int64_t first, int64_t stride, int c0, int lanes, int dim) {
+    threads = L == 0 ? (int)blockDim.x : 256;
+    mine = reinterpret_cast<char*>(smem + (size_t)part * S * C * threads + threadIdx.x);
+    from = reinterpret_cast<const char*>(reinterpret_cast<const T*>(base) + first * ld + c0);
+    row_bytes = stride * ld * (int64_t)sizeof(T);
+    left = (dim - c0) * (int)sizeof(T);
+    advance = 16 * lanes;
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance, left = (dim - c) * (int)sizeof(T);
-      const int bytes = EDGE ? max(0, min(16, left)) : (left > 0 ? 16 : 0);
-      copy_async(mine + (slot * C + k) * threads, row + (bytes > 0 ? c : c0), bytes);
-    }
+    for (int i = 0; i < S * C; ++i)
+      if (i % C * advance >= left) *reinterpret_cast<uint4*>(mine + i * threads * 16) = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void read(int slot, Pack<T> (&out)[C], int c0) const {
+  // The next row into the slot at byte `at`.  What lies behind it is zero.  In front of it (c0 < 0) the vector holds what
+  // the 16 bytes hold: the end of the row before, or what precedes the matrix in its allocation; read() clears it.
+  __device__ __forceinline__ void fetch(int at) {
 #pragma unroll
-    for (int k = 0; k < C; ++k) out[k].raw = mine[(slot * C + k) * threads];
+    for (int k = 0; k < C; ++k)
+      if (k * advance < left)
+        copy_async(reinterpret_cast<uint4*>(mine + at + k * threads * 16), from + k * advance, EDGE ? min(16, left - k * advance) : 16);
+    from += row_bytes;
+  }
+  __device__ __forceinline__ void read(int at, Pack<T> (&out)[C], int c0) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) out[k].raw = *reinterpret_cast<const uint4*>(mine + at + k * threads * 16);
     if (EDGE && c0 < 0) {
 #pragma unroll
       for (int t = 0; t < kVec<T>; ++t)
         if (c0 + t < 0) out[0].v[t] = from_float<T>(0.0f);
     }
   }
+  // bytes from a slot to the next, and the slots' end
+  __device__ __forceinline__ int slot_bytes() const { return C * threads * 16; }
 };
+
+// 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place
+__device__ __forceinline__ float rsqrt_of(float v) {
+  const float r = rsqrtf(v);
+  return __fmaf_rn(0.5f * r, __fmaf_rn(-(v * r), r, 1.0f), r);
+}
 
 // Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }

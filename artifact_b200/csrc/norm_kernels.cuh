@@ -46,6 +46,11 @@ __device__ __forceinline__ void load_columns(float2 (&out)[C][kVec<T> / 2], cons
     }
 }
 
+// how many rows first, first + stride, ... there are
+__device__ __forceinline__ int rows_of(int64_t rows, int64_t first, int64_t stride) {
+  return first < rows ? (int)((rows - first + stride - 1) / stride) : 0;
+}
+
 // What is computed from v is computed where it is used: the comparisons of a thread's columns with the ends of the row do not
 // change from row to row, but kept over the loop they cost more registers than the row itself.
 __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v)); }
@@ -63,27 +68,32 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
   const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
   const float inv = 1.0f / (float)a.dim;
   constexpr int S = ring_slots<C>();
-  const Ring<T, C, S, EDGE> ring(ring_memory, 0);
-  const T* x = reinterpret_cast<const T*>(a.x);
+  const int rows = rows_of(a.rows, g.first, g.stride);
+  Ring<T, L, C, S, EDGE> ring(ring_memory, 0, a.x, a.ldx, g.first, g.stride, c0, g.lanes, a.dim);
+  const int slot_bytes = ring.slot_bytes();
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
-    const int64_t r = g.first + i * g.stride;
-    if (r < a.rows) ring.fetch(i, x + r * a.ldx, c0, advance, a.dim);
+    if (i < rows) ring.fetch(i * slot_bytes);
     copy_commit();
   }
   float2 w[C][H], b[C][H];
   load_columns<T, C>(w, a.weight, a.wf32, a.dim, c0, advance, 1.0f);
   load_columns<T, C>(b, a.bias, a.wf32, a.dim, c0, advance, 0.0f);
-  int slot = 0;
-  for (int64_t r = g.first; r < a.rows; r += g.stride) {
+  const bool ragged = EDGE || a.dim != g.lanes * C * V;            // some threads hold less than C vectors of the row
+  int at = 0, next = (S - 1) * slot_bytes;         // the slot to read and the one to fill
+  T* y = reinterpret_cast<T*>(a.out) + g.first * a.ldo;
+  const int64_t y_step = g.stride * a.ldo, e_step = g.stride * a.dim;
+  float2* stats = a.stats != nullptr ? a.stats + g.first : nullptr;
+  int64_t e = HIDDEN ? a.drop.first + g.first * a.dim + c0 : 0;
+  for (int i = 0; i < rows; ++i) {
     if constexpr (EDGE) not_hoisted(c0);
     Pack<T> raw[C];
     copy_wait<S - 2>();
-    ring.read(slot, raw, c0);
-    const int64_t ahead = r + (S - 1) * g.stride;
-    if (ahead < a.rows) ring.fetch(slot == 0 ? S - 1 : slot - 1, x + ahead * a.ldx, c0, advance, a.dim);
+    ring.read(at, raw, c0);
+    if (i + S - 1 < rows) ring.fetch(next);
     copy_commit();
-    slot = slot == S - 1 ? 0 : slot + 1;
+    next = at;
+    at = at == (S - 1) * slot_bytes ? 0 : at + slot_bytes;
     float2 v[C][H], total = both(0.0f);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
@@ -94,16 +104,24 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
     // the mean, corrected by the sum of the deviations from its first value
     float mean = g.sum(total.x + total.y, buf[0]) * inv;
     float2 dev1 = both(0.0f), dev2 = both(0.0f), minus = both(-mean);
+    if (ragged) {                                   // what lies outside the row deviates by nothing
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance;
-      if (c < 0 || c + V > a.dim) {                 // what lies outside the row deviates by nothing
+      for (int k = 0; k < C; ++k) {
+        const int c = c0 + k * advance;
+        if (!EDGE) {
 #pragma unroll
-        for (int t = 0; t < H; ++t) {
-          if ((unsigned)(c + 2 * t) >= (unsigned)a.dim) v[k][t].x = mean;
-          if ((unsigned)(c + 2 * t + 1) >= (unsigned)a.dim) v[k][t].y = mean;
+          for (int t = 0; t < H; ++t) v[k][t] = c < a.dim ? v[k][t] : both(mean);
+        } else if (c < 0 || c + V > a.dim) {
+#pragma unroll
+          for (int t = 0; t < H; ++t) {
+            if ((unsigned)(c + 2 * t) >= (unsigned)a.dim) v[k][t].x = mean;
+            if ((unsigned)(c + 2 * t + 1) >= (unsigned)a.dim) v[k][t].y = mean;
+          }
         }
       }
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
 #pragma unroll
       for (int t = 0; t < H; ++t) {
         const float2 d = __fadd2_rn(v[k][t], minus);
@@ -115,8 +133,11 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
     const float off = dev.x * inv;
     mean += off;
     minus = both(-mean);
-    const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
-    if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+    const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    if (stats != nullptr) {
+      if (g.lane == 0) *stats = make_float2(mean, rstd);
+      stats += g.stride;
+    }
 #pragma unroll
     for (int k = 0; k < C; ++k)
 #pragma unroll
@@ -130,7 +151,8 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
       }
       if (a.drop.on) {
         uint32_t words[C * V];
-        draw_words<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, words);
+        draw_words<C, V, EDGE>(a.drop, step, e, advance, words);
+        e += e_step;
         scale_elements(v, a.drop.scale);
 #pragma unroll
         for (int k = 0; k < C; ++k)
@@ -138,10 +160,10 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_block
           for (int t = 0; t < H; ++t) v[k][t] = kept_of(a.drop, words + k * V + 2 * t, v[k][t]);
       }
     }
-    T* y = reinterpret_cast<T*>(a.out) + r * a.ldo;
 #pragma unroll
     for (int k = 0; k < C; ++k)
       if (c0 + k * advance < a.dim) store_vec<T, EDGE>(y, c0 + k * advance, a.dim, v[k]);
+    y += y_step;
   }
 }
 
@@ -191,19 +213,20 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
   const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
   const float inv = 1.0f / (float)a.dim;
   constexpr int S = ring_slots<C>();
-  const Ring<T, C, S, EDGE> ring_x(ring_memory, 0), ring_dy(ring_memory, 1);
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* dy = reinterpret_cast<const T*>(a.dy);
+  const int rows = rows_of(a.rows, g.first, g.stride);
+  Ring<T, L, C, S, EDGE> ring_x(ring_memory, 0, a.x, a.ldx, g.first, g.stride, c0, g.lanes, a.dim);
+  Ring<T, L, C, S, EDGE> ring_dy(ring_memory, 1, a.dy, a.lddy, g.first, g.stride, c0, g.lanes, a.dim);
+  const int slot_bytes = ring_x.slot_bytes();
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
-    const int64_t r = g.first + i * g.stride;
-    if (r < a.rows) {
-      ring_x.fetch(i, x + r * a.ldx, c0, advance, a.dim);
-      ring_dy.fetch(i, dy + r * a.lddy, c0, advance, a.dim);
+    if (i < rows) {
+      ring_x.fetch(i * slot_bytes);
+      ring_dy.fetch(i * slot_bytes);
     }
     copy_commit();
   }
-  float2 st_next = g.first < a.rows ? a.stats[g.first] : both(0.0f);
+  const float2* stats = a.stats + g.first;
+  float2 st_next = rows > 0 ? *stats : both(0.0f);
   float2 w[C][H], b[HIDDEN ? C : 1][H], aw[C][H], ab[C][H];
   load_columns<T, C>(w, a.weight, a.wf32, a.dim, c0, advance, 1.0f);
   if constexpr (HIDDEN) load_columns<T, C>(b, a.relu ? a.bias : nullptr, a.wf32, a.dim, c0, advance, 0.0f);
@@ -211,26 +234,31 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
   for (int k = 0; k < C; ++k)
 #pragma unroll
     for (int t = 0; t < H; ++t) aw[k][t] = ab[k][t] = both(0.0f);
-  int turn = 0, slot = 0;
-  for (int64_t r = g.first; r < a.rows; r += g.stride, turn ^= 1) {
+  int turn = 0, at = 0, next = (S - 1) * slot_bytes;
+  T* dx = reinterpret_cast<T*>(a.out) + g.first * a.ldo;
+  const int64_t dx_step = g.stride * a.ldo, e_step = g.stride * a.dim;
+  int64_t e = HIDDEN ? a.drop.first + g.first * a.dim + c0 : 0;
+  for (int i = 0; i < rows; ++i, turn ^= 1) {
     if constexpr (EDGE) not_hoisted(c0);
     const float2 st = st_next;
-    if (r + g.stride < a.rows) st_next = a.stats[r + g.stride];
+    stats += g.stride;
+    if (i + 1 < rows) st_next = *stats;
     uint32_t words[HIDDEN ? C * V : 1];             // drawn while the row is on its way
     if constexpr (HIDDEN) {
-      if (a.drop.on) draw_words<C, V, EDGE>(a.drop, step, a.drop.first + r * a.dim + c0, advance, words);
+      if (a.drop.on) draw_words<C, V, EDGE>(a.drop, step, e, advance, words);
+      e += e_step;
     }
     Pack<T> rx[C], rd[C];
     copy_wait<S - 2>();
-    ring_x.read(slot, rx, c0);
-    ring_dy.read(slot, rd, c0);
-    const int64_t ahead = r + (S - 1) * g.stride;
-    if (ahead < a.rows) {
-      ring_x.fetch(slot == 0 ? S - 1 : slot - 1, x + ahead * a.ldx, c0, advance, a.dim);
-      ring_dy.fetch(slot == 0 ? S - 1 : slot - 1, dy + ahead * a.lddy, c0, advance, a.dim);
+    ring_x.read(at, rx, c0);
+    ring_dy.read(at, rd, c0);
+    if (i + S - 1 < rows) {
+      ring_x.fetch(next);
+      ring_dy.fetch(next);
     }
     copy_commit();
-    slot = slot == S - 1 ? 0 : slot + 1;
+    next = at;
+    at = at == (S - 1) * slot_bytes ? 0 : at + slot_bytes;
     const float2 minus = both(-st.x), rstd = both(st.y);
     float2 h[C][H], gr[C][H], s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
@@ -266,7 +294,6 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
       }
     }
     if (a.out == nullptr) continue;
-    T* dx = reinterpret_cast<T*>(a.out) + r * a.ldo;
     const float2 sums = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), buf[turn]);
     const float2 c1 = both(-sums.x * inv), c2 = both(-sums.y * inv);
 #pragma unroll
@@ -278,6 +305,7 @@ __global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_bloc
       for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(__fadd2_rn(gr[k][t], __ffma2_rn(h[k][t], c2, c1)), rstd);
       store_vec<T, EDGE>(dx, c, a.dim, o);
     }
+    dx += dx_step;
   }
   if (a.partial != nullptr) {
     copy_wait<0>();                                 // the groups' sums go where the ring was
@@ -333,7 +361,7 @@ __global__ void __launch_bounds__(256) norm_forward_plain(const __grid_constant_
     dev = g.sum(dev, buf[1]);
     const float off = dev.x * inv;
     mean += off;
-    const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
     if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
     for (int c = g.lane; c < a.dim; c += g.lanes) {
       float z = affine((to_float(x[c]) - mean) * rstd, a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f,
@@ -633,6 +661,7 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 64) f.template operator()<32, 2>(256);
     else if (vectors <= 96) f.template operator()<32, 3>(256);
     else if (vectors <= 128) f.template operator()<32, 4>(256);
+    else if (vectors <= 1024) return wide_rows<2>(vectors, f);
     else return wide_rows<4>(vectors, f);
   } else if constexpr (MANY) {
     if (vectors <= 4) f.template operator()<4, 1>(256);
@@ -640,6 +669,7 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 16) f.template operator()<16, 1>(256);
     else if (vectors <= 32) f.template operator()<32, 1>(256);
     else if (vectors <= 64) f.template operator()<32, 2>(256);
+    else if (vectors <= 512) return wide_rows<1>(vectors, f);
     else return wide_rows<2>(vectors, f);
   } else if constexpr (sizeof(T) == 4) {                // up to 20 elements per thread
     if (vectors <= 4) f.template operator()<4, 1>(256);

@@ -38,7 +38,7 @@ __device__ __forceinline__ void clear_dropped(const Drop& d, const uint32_t* w, 
 // Blocks per SM that the register allocation aims at: as many as leave nothing spilled.
 template <int MODE, int E>
 constexpr int tile_blocks() {
-  return MODE == kNormBackwardHidden ? (E <= 4 ? 3 : 2) : MODE == kNormBackward ? (E <= 8 ? 3 : 2) : (E <= 8 ? 4 : 3);
+  return MODE == kNormBackwardHidden ? (E <= 4 ? 3 : 2) : MODE == kNormBackward ? (E <= 8 ? 3 : 2) : MODE == kNormForwardHidden ? (E <= 8 ? 3 : E <= 12 ? 3 : 2) : (E <= 8 ? 4 : 3);
 }
 
 // E elements per thread.  Pair j of lane i holds columns c, c + 1 with c = 2 (i + L j) - s: s = 1 for the odd rows of an odd width (ODD),
@@ -59,7 +59,12 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
   const int dim = a.dim, tid = threadIdx.x;
   const int vectors = R * dim / V;                  // of a whole tile
   const bool second = kBack && a.b != nullptr;
-  const int64_t tiles = (a.rows + R - 1) / R, whole = a.rows / R;
+  // this block's tiles, whole ones first
+  const int64_t all_tiles = (a.rows + R - 1) / R, whole_tiles = a.rows / R;
+  const int tiles = blockIdx.x < all_tiles ? (int)((all_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
+  const int whole = blockIdx.x < whole_tiles ? (int)((whole_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
+  const int last = (int)(a.rows - whole_tiles * R) * dim;        // elements of the matrix's last tile, where it is not whole
+  constexpr int kSureM = R * (FEWEST + 1) / V / 256;             // every thread has this many vectors of a tile
   const uint64_t step = step_of(a.drop);
   const bool draw_in = (MODE == kNormBackwardHidden && a.drop.on) || (MODE == kDropBackward && a.drop.on && !a.relu);
   const bool draw_out = (MODE == kNormForwardHidden || MODE == kDropForward) && a.drop.on;
@@ -67,21 +72,35 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
   const int s = ODD ? (g.index * dim) & 1 : 0;
   const int c0 = 2 * g.lane - s;                    // the column of pair j is c0 + 2 L j
 
-  const auto slot_at = [&](int slot, int which) { return tile_memory + (slot * (kBack ? 2 : 1) + which) * vectors; };
-  // brings tile t into a slot; what lies behind the matrix is zero
-  const auto fetch = [&](int64_t t, int slot) {
-    const int64_t first = t * (R * dim);
-    const T* pa = reinterpret_cast<const T*>(a.a) + first;
-    const T* pb = reinterpret_cast<const T*>(a.b) + first;
-    const int n = t < whole ? vectors * 16 : (int)((a.rows * dim - first) * (int)sizeof(T));
+  const int slot_bytes = (kBack ? 2 : 1) * vectors * 16;
+  char* const memory = reinterpret_cast<char*>(tile_memory);
+  const int64_t tile0 = (int64_t)blockIdx.x * (R * dim), tile_step = (int64_t)gridDim.x * (R * dim);   // in elements
+  const T* from_a = reinterpret_cast<const T*>(a.a) + tile0 + tid * V;
+  const T* from_b = reinterpret_cast<const T*>(a.b) + tile0 + tid * V;
+  const auto mine = [&](int m, int n) { return m < kSureM || m * 256 + tid < n; };
+  // brings the next tile, the i-th, into the slot at byte `at`; what lies behind the matrix is zero
+  const auto fetch = [&](int i, int at) {
+    uint4* pa = reinterpret_cast<uint4*>(memory + at) + tid;
+    uint4* pb = pa + vectors;
+    if (i < whole) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const int i = m * 256 + tid;
-      if (i * 16 < n) {
-        copy_async(slot_at(slot, 0) + i, pa + i * V, min(16, n - i * 16));
-        if (second) copy_async(slot_at(slot, 1) + i, pb + i * V, min(16, n - i * 16));
+      for (int m = 0; m < M; ++m)
+        if (mine(m, vectors)) {
+          copy_async(pa + m * 256, from_a + m * 256 * V, 16);
+          if (second) copy_async(pb + m * 256, from_b + m * 256 * V, 16);
+        }
+    } else {
+#pragma unroll 1
+      for (int m = 0; m < M; ++m) {
+        const int bytes = min(16, (last - (m * 256 + tid) * V) * (int)sizeof(T));
+        if (bytes > 0) {
+          copy_async(pa + m * 256, from_a + m * 256 * V, bytes);
+          if (second) copy_async(pb + m * 256, from_b + m * 256 * V, bytes);
+        }
       }
     }
+    from_a += tile_step;
+    from_b += tile_step;
   };
   // a row's pairs in shared memory
   const auto read = [&](const T* row, float2 (&v)[P]) {
@@ -106,13 +125,14 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
 
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
-    const int64_t t = blockIdx.x + (int64_t)i * gridDim.x;
-    if (t < tiles) fetch(t, i);
+    if (i < tiles) fetch(i, i * slot_bytes);
     copy_commit();
   }
+  float2* stats = a.stats + g.first;
+  const int64_t row_step = (int64_t)gridDim.x * R;
   float2 st_next = both(0.0f);
   if constexpr (kNorm && kBack) {
-    if (g.first < a.rows) st_next = a.stats[g.first];
+    if (g.first < a.rows) st_next = *stats;
   }
   float2 w[kWeight ? P : 1], b[kBias ? P : 1], aw[kNorm && kBack ? P : 1], ab[kBack ? P : 1];
 #pragma unroll
@@ -130,24 +150,24 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
     if constexpr (kBack) ab[j] = both(0.0f);
   }
 
-  int slot = 0;
-  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t r = t * R + g.index;
-    const bool live = t < whole || r < a.rows;
+  int at = 0, next = (S - 1) * slot_bytes;
+  T* out = reinterpret_cast<T*>(a.out) + tile0 + tid * V;
+  int64_t e = a.drop.first + tile0 + tid * V;
+  for (int i = 0; i < tiles; ++i) {
+    const bool live = i < whole || g.index * dim < last;
     const float2 st = st_next;
     if constexpr (kNorm && kBack) {
-      const int64_t ahead = r + (int64_t)gridDim.x * R;
-      if (ahead < a.rows) st_next = a.stats[ahead];
+      if (i + 1 < whole || (i + 1 < tiles && g.index * dim < last)) st_next = stats[row_step];
     }
     if constexpr (MODE == kNormBackwardHidden || MODE == kDropBackward) {
       if (draw_in) {                                // on the vectors that this thread copied itself
         uint32_t words[M * V];
-        draw_words<M, V, true>(a.drop, step, a.drop.first + t * (R * dim) + tid * V, 256 * V, words);
+        draw_words<M, V, true>(a.drop, step, e, 256 * V, words);
         copy_wait<S - 2>();
-        uint4* p = slot_at(slot, kNorm ? 1 : 0) + tid;
+        uint4* p = reinterpret_cast<uint4*>(memory + at) + (kNorm ? vectors : 0) + tid;
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          if (m * 256 + tid < vectors) {
+          if (mine(m, vectors)) {
             uint4 raw = p[m * 256];
             clear_dropped<T>(a.drop, words + m * V, raw);
             p[m * 256] = raw;
@@ -157,12 +177,11 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
     }
     copy_wait<S - 2>();
     __syncthreads();                                // the tile is complete, and the slot before it is free
-    const int64_t later = t + (int64_t)(S - 1) * gridDim.x;
-    if (later < tiles) fetch(later, slot == 0 ? S - 1 : slot - 1);
+    if (i + S - 1 < tiles) fetch(i + S - 1, next);
     copy_commit();
 
-    T* pa = reinterpret_cast<T*>(slot_at(slot, 0)) + g.index * dim;
-    const T* pb = reinterpret_cast<const T*>(slot_at(slot, kBack ? 1 : 0)) + g.index * dim;
+    T* pa = reinterpret_cast<T*>(memory + at) + g.index * dim;
+    const T* pb = reinterpret_cast<const T*>(memory + at + vectors * 16) + g.index * dim;
     if (live) {
       float2 v[P];
       read(pa, v);
@@ -185,8 +204,8 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
         const float off = dev.x * inv;
         mean += off;
         minus = both(-mean);
-        const float rstd = __frsqrt_rn(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
-        if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
+        const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+        if (a.stats != nullptr && g.lane == 0) *stats = make_float2(mean, rstd);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
           float2 z = __ffma2_rn(__fmul2_rn(__fadd2_rn(v[j], minus), both(rstd)), w[j], b[j]);
@@ -249,32 +268,34 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
       }
     }
     if (a.out != nullptr) {
-      const int64_t first = t * (R * dim);
       uint32_t words[kBack ? 1 : M * V];
       if constexpr (!kBack) {
-        if (draw_out) draw_words<M, V, true>(a.drop, step, a.drop.first + first + tid * V, 256 * V, words);
+        if (draw_out) draw_words<M, V, true>(a.drop, step, e, 256 * V, words);
       }
       __syncthreads();                              // the results are complete
-      T* out = reinterpret_cast<T*>(a.out) + first;
-      const uint4* p = slot_at(slot, 0);
-      const int n = t < whole ? vectors : (int)((a.rows * dim - first) / V);
+      const uint4* p = reinterpret_cast<const uint4*>(memory + at) + tid;
+      const int n = i < whole ? vectors : last / V;
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        if (m * 256 + tid < n) {
-          uint4 raw = p[m * 256 + tid];
+        if (i < whole ? mine(m, vectors) : m * 256 + tid < n) {
+          uint4 raw = p[m * 256];
           if constexpr (!kBack) {
             if (draw_out) clear_dropped<T>(a.drop, words + m * V, raw);
           }
-          *reinterpret_cast<uint4*>(out + (m * 256 + tid) * V) = raw;
+          *reinterpret_cast<uint4*>(out + m * 256 * V) = raw;
         }
       // the matrix's last elements that fill no vector
-      if (t >= whole && first + n * V + tid < a.rows * dim) {
-        const int i = n * V + tid;
-        const bool keep = kBack || !draw_out || kept(a.drop, step, a.drop.first + first + i);
-        out[i] = keep ? reinterpret_cast<const T*>(p)[i] : from_float<T>(0.0f);
+      if (i >= whole && tid < last - n * V) {
+        const int64_t off = n * V + tid - tid * V;
+        const bool keep = kBack || !draw_out || kept(a.drop, step, e + off);
+        out[off] = keep ? reinterpret_cast<const T*>(memory + at)[n * V + tid] : from_float<T>(0.0f);
       }
+      out += tile_step;
     }
-    slot = slot == S - 1 ? 0 : slot + 1;
+    e += tile_step;
+    if constexpr (kNorm) stats += row_step;
+    next = at;
+    at = at == (S - 1) * slot_bytes ? 0 : at + slot_bytes;
   }
 
   if constexpr (kBack) {
