@@ -142,13 +142,11 @@ __device__ __forceinline__ uint4 philox7(uint64_t group, uint64_t step, const ui
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
-    // (the halves of a product one by one: 31 lanes a cycle and SM against 26 for the 64-bit product)
-    const uint32_t ah = __umulhi(0xD2511F53u, c0), al = 0xD2511F53u * c0;
-    const uint32_t bh = __umulhi(0xCD9E8D57u, c2), bl = 0xCD9E8D57u * c2;
-    c0 = bh ^ c1 ^ key[2 * r];
-    c2 = ah ^ c3 ^ key[2 * r + 1];
-    c1 = bl;
-    c3 = al;
+    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ key[2 * r];
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ key[2 * r + 1];
+    c1 = (uint32_t)b;
+    c3 = (uint32_t)a;
   }
   return make_uint4(c0, c1, c2, c3);
 }

@@ -23,6 +23,10 @@ __device__ __forceinline__ int row_shift(const void* base, int64_t ld, int64_t r
   return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(r * ld)) % kVec<T>);
 }
 
+// Threads of a block that owns a row: at most this many, so that 16 elements a thread have 128 registers and 32 have 255.
+template <class T, int C>
+constexpr int wide_threads() { return C * kVec<T> <= 16 ? 512 : 256; }
+
 // Blocks of 256 threads per SM that the register allocation aims at: as many as leave nothing spilled.
 template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int forward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN && EDGE ? 3 : 4) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? (HIDDEN && EDGE ? 2 : 3) : HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : 2; }
@@ -57,7 +61,7 @@ __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v))
 
 // HIDDEN: with the ReLU or the dropout (or both)
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN, EDGE>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN, EDGE>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
@@ -202,7 +206,7 @@ __device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2
 
 // dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
 template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? 512 : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, EDGE>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, EDGE>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
@@ -638,20 +642,21 @@ Layout layout_of(int64_t rows, int dim, std::initializer_list<Matrix> all) {
 }
 
 // a block per row
-template <int C, class F>
+template <class T, int C, class F>
 bool wide_rows(int vectors, F&& f) {
   const int threads = ((vectors + C - 1) / C + 31) / 32 * 32;
-  if (threads > 512) return false;
+  if (threads > wide_threads<T, C>()) return false;
   f.template operator()<0, C>(threads);
   return true;
 }
 
 // Group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads).  The
 // fewest lanes whose registers hold the row: they have the most bytes in flight each and the fewest steps in the row's sums.
-// MANY: the backward pass through a ReLU or a dropout also keeps the biases, and gets by with fewer elements a thread.
-template <class T, bool MANY, class F>
+// The backward pass through a ReLU or a dropout also keeps the biases and the words, and gets by with fewer elements a thread.
+enum Pass { kForward, kBackward, kBackwardHidden };
+template <class T, Pass PASS, class F>
 bool by_width(int vectors, F&& f) {
-  if constexpr (MANY && sizeof(T) == 4) {
+  if constexpr (PASS == kBackwardHidden && sizeof(T) == 4) {
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<4, 2>(256);
     else if (vectors <= 16) f.template operator()<8, 2>(256);
@@ -661,17 +666,17 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 64) f.template operator()<32, 2>(256);
     else if (vectors <= 96) f.template operator()<32, 3>(256);
     else if (vectors <= 128) f.template operator()<32, 4>(256);
-    else if (vectors <= 1024) return wide_rows<2>(vectors, f);
-    else return wide_rows<4>(vectors, f);
-  } else if constexpr (MANY) {
+    else if (vectors <= 1024) return wide_rows<T, 2>(vectors, f);
+    else return wide_rows<T, 4>(vectors, f);
+  } else if constexpr (PASS == kBackwardHidden) {
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<8, 1>(256);
     else if (vectors <= 16) f.template operator()<16, 1>(256);
     else if (vectors <= 32) f.template operator()<32, 1>(256);
     else if (vectors <= 64) f.template operator()<32, 2>(256);
-    else if (vectors <= 512) return wide_rows<1>(vectors, f);
-    else return wide_rows<2>(vectors, f);
-  } else if constexpr (sizeof(T) == 4) {                // up to 20 elements per thread
+    else if (vectors <= 512) return wide_rows<T, 1>(vectors, f);
+    else return wide_rows<T, 2>(vectors, f);
+  } else if constexpr (sizeof(T) == 4) {
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<4, 2>(256);
     else if (vectors <= 12) f.template operator()<4, 3>(256);
@@ -686,8 +691,9 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 96) f.template operator()<32, 3>(256);
     else if (vectors <= 128) f.template operator()<32, 4>(256);
     else if (vectors <= 160) f.template operator()<32, 5>(256);
-    else return wide_rows<4>(vectors, f);
-  } else {                                       // up to 24
+    else if (PASS == kForward && vectors <= 256) f.template operator()<32, PASS == kForward ? 8 : 5>(256);
+    else return wide_rows<T, 4>(vectors, f);
+  } else {
     if (vectors <= 4) f.template operator()<4, 1>(256);
     else if (vectors <= 8) f.template operator()<4, 2>(256);
     else if (vectors <= 12) f.template operator()<4, 3>(256);
@@ -697,7 +703,9 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 48) f.template operator()<16, 3>(256);
     else if (vectors <= 64) f.template operator()<32, 2>(256);
     else if (vectors <= 96) f.template operator()<32, 3>(256);
-    else return wide_rows<2>(vectors, f);
+    else if (PASS == kBackward && vectors <= 128) f.template operator()<32, PASS == kBackward ? 4 : 3>(256);
+    else if (PASS == kForward && vectors <= 256) return wide_rows<T, 2>(vectors, f);
+    else return wide_rows<T, 4>(vectors, f);
   }
   return true;
 }
@@ -711,7 +719,7 @@ struct NormForward {
     auto kernel = norm_forward_kernel<T, L, C, HIDDEN, EDGE>;
     constexpr int per_thread = 16 * C * ring_slots<C>();
     static std::atomic<uint64_t> seen{0};
-    allow_smem(kernel, per_thread * (L == 0 ? 512 : 256), seen);
+    allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
     static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
     constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
     int64_t most = (int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full);
@@ -731,7 +739,7 @@ struct NormBackward {
     auto kernel = norm_backward_kernel<T, L, C, HIDDEN, EDGE>;
     constexpr int per_thread = std::max(32 * C * ring_slots<C>(), L == 0 ? 0 : C * kVec<T> * 4);
     static std::atomic<uint64_t> seen{0};
-    allow_smem(kernel, per_thread * (L == 0 ? 512 : 256), seen);
+    allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
     static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
     constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
     const int64_t most = std::min<int64_t>((int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full), column_blocks_cap(a.rows, a.dim));
@@ -776,8 +784,8 @@ cudaError_t launch_norm_forward(const NormArgs& given, cudaStream_t stream) {
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
   bool done = false;
   if (l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T, false>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T, false>(l.vectors, NormForward<T, true, false>{a, stream});
-    else done = l.edge ? by_width<T, false>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T, false>(l.vectors, NormForward<T, false, false>{a, stream});
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T, kForward>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, true, false>{a, stream});
+    else done = l.edge ? by_width<T, kForward>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, false, false>{a, stream});
   }
   if (!done) norm_forward_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
   return cudaGetLastError();
@@ -795,8 +803,8 @@ cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
   }
   const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
   if (!done && l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T, true>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T, true>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
-    else done = l.edge ? by_width<T, false>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T, false>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
+    if (a.drop.on || a.relu) done = l.edge ? by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
+    else done = l.edge ? by_width<T, kBackward>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T, kBackward>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
   }
   if (!done) {
     if (a.out != nullptr) norm_backward_rows_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
