@@ -43,10 +43,11 @@ union Pack {
   __device__ Pack() {}
 };
 
-// columns [c, c + VEC) of a row; what lies outside [0, dim) is zero
+// Columns [c, c + VEC) of a row, c + VEC > 0.  Partial vectors hold what the 16 bytes hold, the neighbouring row's elements or what
+// precedes the matrix in its allocation; behind the end of the matrix (`last`: its last row) nothing is read.
 template <class T, bool EDGE>
-__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim) {
-  if (!EDGE || (c >= 0 && c + kVec<T> <= dim)) {
+__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim, bool last) {
+  if (!EDGE || !last || c + kVec<T> <= dim) {
     out.raw = *reinterpret_cast<const uint4*>(row + c);
   } else {
 #pragma unroll

@@ -509,10 +509,11 @@ __global__ void __launch_bounds__(256, 4) dropout_flat_kernel(const __grid_const
   }
 }
 
-// thread = vector `col` of the rows row0, row0 + stride, ...; a.lanes threads side by side cover a tile of a row
+// Thread = vector `c` of the rows first, first + stride, ...; a.lanes threads side by side cover a tile of a row.  U rows at a time:
+// their loads and their calls of the generator run side by side.
 template <class T, bool BACK, bool DRAW, bool EDGE>
-__global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
-  constexpr int V = kVec<T>, U = 4;
+__global__ void __launch_bounds__(256, 3) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
+  constexpr int V = kVec<T>, U = BACK && !DRAW ? 4 : 16 / V;
   extern __shared__ float columns[];
   const int groups = blockDim.x / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes;
   const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
@@ -532,8 +533,9 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const __grid_constant
       for (int u = 0; u < U; ++u) {
         in[u].raw = yy[u].raw = make_uint4(0, 0, 0, 0);
         if (r + u * stride < a.rows) {
-          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim);
-          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim);
+          const bool last = r + u * stride == a.rows - 1;
+          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim, last);
+          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim, last);
         }
       }
       float2 o[U][V / 2];
@@ -817,6 +819,19 @@ cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
   return launch_join<T>(a.partial, blocks, 2 * a.dim, a.dim, a.dweight, a.dbias, a.wf32, stream);
 }
 
+// As many blocks as run at once; a multiple of 8, so that a thread's rows keep their distance to the 16-byte boundaries.
+template <class T, bool BACK, bool DRAW, bool EDGE>
+int launch_dropout_rows(const DropArgs& a, int groups, int threads, int tiles, int smem, cudaStream_t stream) {
+  auto kernel = dropout_rows_kernel<T, BACK, DRAW, EDGE>;
+  static const int full = blocks_per_sm(kernel, 256, BACK ? 256 * kVec<T> * 4 : 0);
+  int64_t most = (int64_t)kSMs * (full * 256 / threads) / tiles;
+  if (a.partial != nullptr) most = std::min<int64_t>(most, column_blocks_cap(a.rows, a.dim));
+  const int n = clamp_blocks((a.rows + groups - 1) / groups, std::max<int64_t>(most, 8));
+  const int blocks = n < 8 ? 8 : n / 8 * 8;
+  kernel<<<dim3(blocks, tiles), threads, smem, stream>>>(a);
+  return blocks;
+}
+
 template <class T, bool BACK>
 cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
   DropArgs a = given;
@@ -844,15 +859,11 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
   } else if (l.vec && tiles <= 65535) {
     a.lanes = std::min(l.vectors, 256);
     const int groups = 256 / a.lanes, threads = (groups * a.lanes + 31) / 32 * 32;
-    const int64_t most = a.partial != nullptr ? column_blocks_cap(a.rows, a.dim) : kMaxColumnBlocks;
-    blocks = clamp_blocks((a.rows + groups - 1) / groups, std::max<int64_t>(most / tiles, 8));
-    blocks = blocks < 8 ? 8 : blocks / 8 * 8;
     const int smem = BACK && a.partial != nullptr ? groups * a.lanes * V * 4 : 0;
-    const dim3 grid(blocks, tiles);
-    if (draw && l.edge) dropout_rows_kernel<T, BACK, true, true><<<grid, threads, smem, stream>>>(a);
-    else if (draw) dropout_rows_kernel<T, BACK, true, false><<<grid, threads, smem, stream>>>(a);
-    else if (l.edge) dropout_rows_kernel<T, BACK, false, true><<<grid, threads, smem, stream>>>(a);
-    else dropout_rows_kernel<T, BACK, false, false><<<grid, threads, smem, stream>>>(a);
+    if (draw && l.edge) blocks = launch_dropout_rows<T, BACK, true, true>(a, groups, threads, tiles, smem, stream);
+    else if (draw) blocks = launch_dropout_rows<T, BACK, true, false>(a, groups, threads, tiles, smem, stream);
+    else if (l.edge) blocks = launch_dropout_rows<T, BACK, false, true>(a, groups, threads, tiles, smem, stream);
+    else blocks = launch_dropout_rows<T, BACK, false, false>(a, groups, threads, tiles, smem, stream);
   } else {
     if (a.out != nullptr) dropout_plain<T, BACK><<<clamp_blocks((a.rows * a.dim + 255) / 256, kSMs * 8), 256, 0, stream>>>(a);
     if (BACK && a.partial != nullptr) {
