@@ -31,11 +31,9 @@ def _check_matrix(x, name):
 
 
 def _check_vector(v, name, x):
-    if v is None:
-        return
     if not isinstance(v, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if v.device != x.device or v.dim() != 1 or v.size(0) != x.size(-1):
+    if v.get_device() != x.get_device() or v.dim() != 1 or v.size(0) != x.size(-1):
         raise RuntimeError(f"{name} must be a vector of {x.size(-1)} entries on x's device, got {tuple(v.shape)} on {v.device}")
     if v.dtype is not torch.float32 and v.dtype is not x.dtype:
         raise RuntimeError(f"{name} must be float32 or of x's type, got {v.dtype}")
@@ -111,20 +109,20 @@ def _call(function, x, *args):
 
 
 def _like(x):
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _workspace(lib, rows, width, x):
     # torch's caching allocator returns 512-byte aligned blocks
     n = lib.rof_layer_norm_workspace_bytes(rows, width)
-    return torch.empty(n, dtype=torch.uint8, device=x.device), n
+    return x.new_empty(n, dtype=torch.uint8), n
 
 
 def _norm_forward(x, weight, bias, eps, relu, drop, want_stats):
     v = _rows(x)
     rows, width = v.shape
     y = _like(x)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if want_stats else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     kind = _kind(weight, bias, x)
     w, b = _vector(weight, kind), _vector(bias, kind)
     _call(_native.cuda().rof_layer_norm_forward, x, DTYPES[x.dtype], v.data_ptr(), v.stride(0), rows, width, DTYPES[kind],
@@ -185,8 +183,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None
     dropout behind it (see `dropout`), only where `training`.  Returns a contiguous tensor like x; gradients flow to x, weight
     and bias (once: a second derivative is not offered)."""
     _check_matrix(x, "x")
-    _check_vector(weight, "weight", x)
-    _check_vector(bias, "bias", x)
+    if weight is not None:
+        _check_vector(weight, "weight", x)
+    if bias is not None:
+        _check_vector(bias, "bias", x)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     drop = _check_drop(p, seed, step, row_offset, training, x)
@@ -250,7 +250,8 @@ def dropout(x, p=0.0, seed=None, step=0, row_offset=0, training=True, bias=None,
     `training`; p = 1 zeroes everything.  The choice depends on (seed, step, element index) alone, the index counted from
     row `row_offset` of the whole matrix.  Returns a contiguous tensor like x."""
     _check_matrix(x, "x")
-    _check_vector(bias, "bias", x)
+    if bias is not None:
+        _check_vector(bias, "bias", x)
     drop = _check_drop(p, seed, step, row_offset, training, x)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _Dropout.apply(x, bias, bool(relu), drop, drop[3] if drop else None)
