@@ -82,6 +82,14 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ void pair_copy(float* to, const float* from) { *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(from); }
+__device__ __forceinline__ void pair_copy(__nv_bfloat16* to, const __nv_bfloat16* from) { *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from); }
+__device__ __forceinline__ void pair_copy(__half* to, const __half* from) { *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from); }
+
+__device__ __forceinline__ void four_copy(float* to, const float* from) { *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(from); }
+template <class T>
+__device__ __forceinline__ void four_copy(T* to, const T* from) { *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from); }
+
 // A thread's own ring of S slots in shared memory for the C vectors of its next rows.  Every thread reads only what it copied
 // itself, so the ring needs no barrier: it is an extension of the registers that keeps (S - 1) C vectors a thread in
 // flight whatever the compiler does with the loads.  A slot is refilled one row after it was read.  Vectors that lie behind the
@@ -125,8 +133,36 @@ struct Ring {
         if (c0 + t < 0) out[0].v[t] = from_float<T>(0.0f);
     }
   }
-  // bytes from a slot to the next, and the slots' end
   __device__ __forceinline__ int slot_bytes() const { return C * threads * 16; }
+  // Stores a row whose output lies differently against the 16-byte boundaries than its input: the group's vectors go into the
+  // slot that was just read, and out of it element by element (W at a time), neighbours by neighbouring lanes.
+  template <int W, class G>
+  __device__ __forceinline__ void store_through(int at, const float2 (&v)[C][kVec<T> / 2], const G& g, T* out, int shift, int dim) const {
+    constexpr int V = kVec<T>;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      Pack<T> p;
+#pragma unroll
+      for (int t = 0; t < V / 2; ++t) pack_two(&p.v[2 * t], v[k][t]);
+      if (k * advance < left) *reinterpret_cast<uint4*>(mine + at + k * threads * 16) = p.raw;   // (the others stay cleared)
+    }
+    g.sync();
+    // vector i of the row is vector i % lanes of the group's slice number i / lanes
+    const T* slot = reinterpret_cast<const T*>(mine + at - g.lane * 16);
+#pragma unroll
+    for (int j = 0; j < C * V / W; ++j) {
+      const int c = (g.lane + j * g.lanes) * W, e = c + shift, i = e / V;
+      if (c < dim) {
+        int k = 0;
+#pragma unroll
+        for (int q = 1; q < C; ++q) k += i >= q * g.lanes;
+        const T* from = slot + (k * threads + (i - k * g.lanes)) * V + e % V;
+        if constexpr (W == 2) pair_copy(out + c, from);
+        else out[c] = *from;
+      }
+    }
+    g.sync();
+  }
 };
 
 // 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place
@@ -249,6 +285,10 @@ struct Group {
       first = (int64_t)blockIdx.x * (blockDim.x / L) + index;
       stride = (int64_t)gridDim.x * (blockDim.x / L);
     }
+  }
+  __device__ __forceinline__ void sync() const {
+    if constexpr (L == 0) __syncthreads();
+    else __syncwarp(mask);
   }
   // Sums over the group, the same in every lane, always added in the same order.  `buf`: two floats per warp, another one
   // for each of two sums that follow one another (L = 0 only).

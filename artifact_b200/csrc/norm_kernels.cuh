@@ -23,6 +23,10 @@ __device__ __forceinline__ int row_shift(const void* base, int64_t ld, int64_t r
   return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(r * ld)) % kVec<T>);
 }
 
+// How the rows of the matrices lie: whole 16-byte vectors; with partial vectors at the ends, the same in all of them; or the inputs
+// alike and the output differently.
+enum { kWhole, kEdges, kMoved };
+
 // Threads of a block that owns a row: at most this many, so that 16 elements a thread have 128 registers and 32 have 255.
 template <class T, int C>
 constexpr int wide_threads() { return C * kVec<T> <= 16 ? 512 : 256; }
@@ -60,9 +64,10 @@ __device__ __forceinline__ int rows_of(int64_t rows, int64_t first, int64_t stri
 __device__ __forceinline__ void not_hoisted(int& v) { asm volatile("" : "+r"(v)); }
 
 // HIDDEN: with the ReLU or the dropout (or both)
-template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN, EDGE>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
+template <class T, int L, int C, bool HIDDEN, int LAYOUT>
+__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : forward_blocks<T, C, HIDDEN, LAYOUT != kWhole>()) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
+  constexpr bool EDGE = LAYOUT != kWhole;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
   const Group<L> g;
@@ -86,6 +91,8 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
   const bool ragged = EDGE || a.dim != g.lanes * C * V;            // some threads hold less than C vectors of the row
   int at = 0, next = (S - 1) * slot_bytes;         // the slot to read and the one to fill
   T* y = reinterpret_cast<T*>(a.out) + g.first * a.ldo;
+  // two elements at a time where both sides allow it
+  const bool pairs = LAYOUT == kMoved && a.dim % 2 == 0 && s % 2 == 0 && a.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % (2 * sizeof(T)) == 0;
   const int64_t y_step = g.stride * a.ldo, e_step = g.stride * a.dim;
   float2* stats = a.stats != nullptr ? a.stats + g.first : nullptr;
   int64_t e = HIDDEN ? a.drop.first + g.first * a.dim + c0 : 0;
@@ -164,9 +171,14 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
           for (int t = 0; t < H; ++t) v[k][t] = kept_of(a.drop, words + k * V + 2 * t, v[k][t]);
       }
     }
+    if constexpr (LAYOUT == kMoved) {
+      if (pairs) ring.template store_through<2>(next, v, g, y, s, a.dim);
+      else ring.template store_through<1>(next, v, g, y, s, a.dim);
+    } else {
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (c0 + k * advance < a.dim) store_vec<T, EDGE>(y, c0 + k * advance, a.dim, v[k]);
+      for (int k = 0; k < C; ++k)
+        if (c0 + k * advance < a.dim) store_vec<T, EDGE>(y, c0 + k * advance, a.dim, v[k]);
+    }
     y += y_step;
   }
 }
@@ -205,9 +217,10 @@ __device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2
 }
 
 // dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
-template <class T, int L, int C, bool HIDDEN, bool EDGE>
-__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, EDGE>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+template <class T, int L, int C, bool HIDDEN, int LAYOUT>
+__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, LAYOUT != kWhole>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
+  constexpr bool EDGE = LAYOUT != kWhole;
   __shared__ float buf[2][32];
   extern __shared__ uint4 ring_memory[];
   const Group<L> g;
@@ -240,6 +253,7 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
     for (int t = 0; t < H; ++t) aw[k][t] = ab[k][t] = both(0.0f);
   int turn = 0, at = 0, next = (S - 1) * slot_bytes;
   T* dx = reinterpret_cast<T*>(a.out) + g.first * a.ldo;
+  const bool pairs = LAYOUT == kMoved && a.dim % 2 == 0 && s % 2 == 0 && a.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % (2 * sizeof(T)) == 0;
   const int64_t dx_step = g.stride * a.ldo, e_step = g.stride * a.dim;
   int64_t e = HIDDEN ? a.drop.first + g.first * a.dim + c0 : 0;
   for (int i = 0; i < rows; ++i, turn ^= 1) {
@@ -301,13 +315,16 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
     const float2 sums = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), buf[turn]);
     const float2 c1 = both(-sums.x * inv), c2 = both(-sums.y * inv);
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      const int c = c0 + k * advance;
-      if (c >= a.dim) continue;
-      float2 o[H];
+    for (int k = 0; k < C; ++k)
 #pragma unroll
-      for (int t = 0; t < H; ++t) o[t] = __fmul2_rn(__fadd2_rn(gr[k][t], __ffma2_rn(h[k][t], c2, c1)), rstd);
-      store_vec<T, EDGE>(dx, c, a.dim, o);
+      for (int t = 0; t < H; ++t) gr[k][t] = __fmul2_rn(__fadd2_rn(gr[k][t], __ffma2_rn(h[k][t], c2, c1)), rstd);
+    if constexpr (LAYOUT == kMoved) {
+      if (pairs) ring_x.template store_through<2>(next, gr, g, dx, s, a.dim);
+      else ring_x.template store_through<1>(next, gr, g, dx, s, a.dim);
+    } else {
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (c0 + k * advance < a.dim) store_vec<T, EDGE>(dx, c0 + k * advance, a.dim, gr[k]);
     }
     dx += dx_step;
   }
@@ -576,23 +593,51 @@ __global__ void __launch_bounds__(256, 3) dropout_rows_kernel(const __grid_const
   }
 }
 
+// Any layout: a thread takes the four elements of a call of the generator (fewer at the matrix's ends), U times; they may lie in two
+// rows or more.  `whole`: bit 0: x, bit 1: y, bit 2: out are contiguous and their groups of four aligned to their size.
 template <class T, bool BACK>
-__global__ void __launch_bounds__(256) dropout_plain(const __grid_constant__ DropArgs a) {
+__global__ void __launch_bounds__(256, 4) dropout_any_kernel(const __grid_constant__ DropArgs a, int whole) {
+  constexpr int U = 2;
   const uint64_t step = step_of(a.drop);
-  const int64_t n = a.rows * a.dim, stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-    const int64_t r = i / a.dim;
-    const int c = (int)(i - r * a.dim);
-    float z = to_float(reinterpret_cast<const T*>(a.x)[r * a.ldx + c]);
-    const bool two = BACK && a.relu;
-    bool keep = !a.drop.on || two || kept(a.drop, step, a.drop.first + i);
-    if constexpr (BACK) {
-      keep = keep && !(two && to_float(reinterpret_cast<const T*>(a.y)[r * a.ldy + c]) <= 0.0f);
-    } else {
-      if (a.bias != nullptr) z += vector_at<T>(a.bias, a.bf32, c);
-      if (a.relu) z = relu_of(z);
+  const bool two = BACK && a.relu, draw = a.drop.on && !two;
+  const int64_t n = a.rows * a.dim, ahead = a.drop.first & 3;         // element 0 is number `ahead` of its group
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i0 = (((int64_t)blockIdx.x * U + u) * 256 + threadIdx.x) * 4 - ahead;
+    if (i0 >= n) return;
+    const int from = i0 < 0 ? (int)-i0 : 0, to = (int)min((int64_t)4, n - i0);
+    int64_t r = (i0 + from) / a.dim;
+    int c = (int)(i0 + from - r * a.dim);
+    const bool full = from == 0 && to == 4;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (draw) w = philox7((uint64_t)(a.drop.first + i0) >> 2, step, a.drop.key);
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    alignas(16) T in[4];
+    alignas(16) T y[4];
+    alignas(16) T out[4];
+    if (full && (whole & 1)) four_copy(in, reinterpret_cast<const T*>(a.x) + i0);
+    if (full && two && (whole & 2)) four_copy(y, reinterpret_cast<const T*>(a.y) + i0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t < from || t >= to) continue;
+      if (!(full && (whole & 1))) in[t] = reinterpret_cast<const T*>(a.x)[r * a.ldx + c];
+      if (two && !(full && (whole & 2))) y[t] = reinterpret_cast<const T*>(a.y)[r * a.ldy + c];
+      float z = to_float(in[t]);
+      if constexpr (BACK) {
+        if (two && to_float(y[t]) <= 0.0f) z = 0.0f;
+      } else {
+        if (a.bias != nullptr) z += vector_at<T>(a.bias, a.bf32, c);
+        if (a.relu) z = relu_of(z);
+      }
+      z *= a.drop.scale;
+      out[t] = from_float<T>(draw && words[t] <= a.drop.last ? 0.0f : z);
+      if (!(full && (whole & 4))) reinterpret_cast<T*>(a.out)[r * a.ldo + c] = out[t];
+      if (++c == a.dim) {
+        c = 0;
+        ++r;
+      }
     }
-    reinterpret_cast<T*>(a.out)[r * a.ldo + c] = from_float<T>(keep ? z * a.drop.scale : 0.0f);
+    if (full && (whole & 4)) four_copy(reinterpret_cast<T*>(a.out) + i0, out);
   }
 }
 
@@ -712,13 +757,13 @@ bool by_width(int vectors, F&& f) {
   return true;
 }
 
-template <class T, bool HIDDEN, bool EDGE>
+template <class T, bool HIDDEN, int LAYOUT>
 struct NormForward {
   const NormArgs& a;
   cudaStream_t stream;
   template <int L, int C>
   void operator()(int threads) const {
-    auto kernel = norm_forward_kernel<T, L, C, HIDDEN, EDGE>;
+    auto kernel = norm_forward_kernel<T, L, C, HIDDEN, LAYOUT>;
     constexpr int per_thread = 16 * C * ring_slots<C>();
     static std::atomic<uint64_t> seen{0};
     allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
@@ -731,14 +776,14 @@ struct NormForward {
   }
 };
 
-template <class T, bool HIDDEN, bool EDGE>
+template <class T, bool HIDDEN, int LAYOUT>
 struct NormBackward {
   const NormArgs& a;
   cudaStream_t stream;
   int* blocks;
   template <int L, int C>
   void operator()(int threads) const {
-    auto kernel = norm_backward_kernel<T, L, C, HIDDEN, EDGE>;
+    auto kernel = norm_backward_kernel<T, L, C, HIDDEN, LAYOUT>;
     constexpr int per_thread = std::max(32 * C * ring_slots<C>(), L == 0 ? 0 : C * kVec<T> * 4);
     static std::atomic<uint64_t> seen{0};
     allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
@@ -783,12 +828,12 @@ cudaError_t launch_norm_forward(const NormArgs& given, cudaStream_t stream) {
     const RowRunArgs t{a.x, nullptr, a.out, a.weight, a.bias, a.wf32, a.stats, nullptr, a.rows, a.dim, a.eps, a.relu, a.drop};
     return tile_launcher(T{})(t, a.relu || a.drop.on ? kNormForwardHidden : kNormForward, stream, nullptr);
   }
-  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
-  bool done = false;
-  if (l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T, kForward>(l.vectors, NormForward<T, true, true>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, true, false>{a, stream});
-    else done = l.edge ? by_width<T, kForward>(l.vectors, NormForward<T, false, true>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, false, false>{a, stream});
-  }
+  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}}), all = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.out, a.ldo}});
+  const bool hidden = a.relu || a.drop.on;
+  bool done;
+  if (!all.vec) done = hidden ? by_width<T, kForward>(l.vectors, NormForward<T, true, kMoved>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, false, kMoved>{a, stream});
+  else if (l.edge) done = hidden ? by_width<T, kForward>(l.vectors, NormForward<T, true, kEdges>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, false, kEdges>{a, stream});
+  else done = hidden ? by_width<T, kForward>(l.vectors, NormForward<T, true, kWhole>{a, stream}) : by_width<T, kForward>(l.vectors, NormForward<T, false, kWhole>{a, stream});
   if (!done) norm_forward_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
@@ -803,10 +848,12 @@ cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
     const cudaError_t e = tile_launcher(T{})(t, a.relu || a.drop.on ? kNormBackwardHidden : kNormBackward, stream, &blocks);
     if (e != cudaSuccess) return e;
   }
-  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
+  const Layout l = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}}), all = layout_of<T>(a.rows, a.dim, {{a.x, a.ldx}, {a.dy, a.lddy}, {a.out, a.ldo}});
+  const bool hidden = a.relu || a.drop.on;
   if (!done && l.vec) {
-    if (a.drop.on || a.relu) done = l.edge ? by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, true>{a, stream, &blocks}) : by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, false>{a, stream, &blocks});
-    else done = l.edge ? by_width<T, kBackward>(l.vectors, NormBackward<T, false, true>{a, stream, &blocks}) : by_width<T, kBackward>(l.vectors, NormBackward<T, false, false>{a, stream, &blocks});
+    if (!all.vec) done = hidden ? by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, kMoved>{a, stream, &blocks}) : by_width<T, kBackward>(l.vectors, NormBackward<T, false, kMoved>{a, stream, &blocks});
+    else if (l.edge) done = hidden ? by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, kEdges>{a, stream, &blocks}) : by_width<T, kBackward>(l.vectors, NormBackward<T, false, kEdges>{a, stream, &blocks});
+    else done = hidden ? by_width<T, kBackwardHidden>(l.vectors, NormBackward<T, true, kWhole>{a, stream, &blocks}) : by_width<T, kBackward>(l.vectors, NormBackward<T, false, kWhole>{a, stream, &blocks});
   }
   if (!done) {
     if (a.out != nullptr) norm_backward_rows_plain<T><<<clamp_blocks(a.rows, kSMs * 8), 256, 0, stream>>>(a);
@@ -865,7 +912,15 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
     else if (l.edge) blocks = launch_dropout_rows<T, BACK, false, true>(a, groups, threads, tiles, smem, stream);
     else blocks = launch_dropout_rows<T, BACK, false, false>(a, groups, threads, tiles, smem, stream);
   } else {
-    if (a.out != nullptr) dropout_plain<T, BACK><<<clamp_blocks((a.rows * a.dim + 255) / 256, kSMs * 8), 256, 0, stream>>>(a);
+    if (a.out != nullptr) {
+      // contiguous, and element i0 of a group lies at a multiple of four elements
+      const auto fours = [&](const void* p, int64_t ld) {
+        return (a.rows == 1 || ld == a.dim) && (reinterpret_cast<uintptr_t>(p) / sizeof(T) - a.drop.first) % 4 == 0;
+      };
+      const int even = (fours(a.x, a.ldx) ? 1 : 0) | (fours(a.y, a.ldy) ? 2 : 0) | (fours(a.out, a.ldo) ? 4 : 0);
+      const int64_t groups = a.rows * a.dim / 4 + 2;
+      dropout_any_kernel<T, BACK><<<(int)((groups + 511) / 512), 256, 0, stream>>>(a, even);
+    }
     if (BACK && a.partial != nullptr) {
       blocks = clamp_blocks((a.rows + 31) / 32, column_blocks_cap(a.rows, a.dim));
       dropout_columns_plain<T><<<dim3((a.dim + 127) / 128, blocks), 128, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);

@@ -103,6 +103,26 @@ def test_rows_views_and_copies():
     assert norm._rows(torch.zeros(2, 3, 0)).shape == (6, 0) and norm._rows(torch.zeros(0, 4)).shape == (0, 4)
 
 
+def test_matrices_are_laid_alike():
+    """a gradient whose rows lie differently against the 16-byte boundaries is copied, one that lies alike is not"""
+    gen = torch.Generator().manual_seed(1)
+    for dtype in (torch.float32, torch.bfloat16):
+        per = 16 // torch.empty(0, dtype=dtype).element_size()
+        flat = torch.randn(4096, generator=gen).to(dtype)
+        start = -flat.data_ptr() // flat.element_size() % per         # an element on a boundary
+        for off in (0, 1, 3):
+            for ld in (12, 13, 14, 16, 40):
+                v = flat.as_strided((7, 11), (ld, 1), start + off)
+                for t in (v, v.contiguous(), flat.as_strided((7, 11), (24, 1), start), flat.as_strided((7, 11), (11, 1), start + 1)):
+                    u = norm._laid_like(t, v)
+                    assert torch.equal(u, t) and u.stride(1) == 1 and u.stride(0) >= 11
+                    for r in range(7):
+                        assert (u[r].data_ptr() - v[r].data_ptr()) % 16 == 0
+                assert norm._laid_like(v, v) is v
+                one = flat.as_strided((1, 11), (3, 1), start + off)
+                assert (norm._laid_like(flat[start + 2:start + 13].view(1, 11), one).data_ptr() - one.data_ptr()) % 16 == 0
+
+
 def test_c_entry_points_refuse_bad_arguments():
     """bad arguments come back as status codes before anything touches a device"""
     lib = _native.cuda()
