@@ -36,9 +36,14 @@ template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int forward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN && EDGE ? 3 : 4) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? (HIDDEN && EDGE ? 2 : 3) : HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : 2; }
 template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 8 : 16) ? 2 : 1; }
-// Slots of the rings
-template <int C>
-constexpr int ring_slots() { return C == 1 ? 4 : C <= 4 ? 3 : 2; }
+// Slots of the rings.  In the forward pass 32-bit rows do best with little in flight (2 slots of 64 bytes a thread and more: 65536x2048 172 us
+// against 191 with 3), 16-bit rows, which take more instructions a byte, with more (16384x4096 51 us with 4, 54 with 3).
+template <class T, int C, bool BACK>
+constexpr int ring_slots() {
+  if (BACK) return C == 1 ? 4 : C <= 4 ? 3 : 2;
+  if (sizeof(T) == 2) return C == 3 ? 3 : 4;
+  return C == 1 ? 4 : C == 2 ? 3 : 2;
+}
 
 // ---- layer norm ---------------------------------------------------------------------------------
 // the thread's entries of a vector (`other` where there is none)
@@ -76,7 +81,7 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
   const int advance = g.lanes * V;
   const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
   const float inv = 1.0f / (float)a.dim;
-  constexpr int S = ring_slots<C>();
+  constexpr int S = ring_slots<T, C, false>();
   const int rows = rows_of(a.rows, g.first, g.stride);
   Ring<T, L, C, S, EDGE> ring(ring_memory, 0, a.x, a.ldx, g.first, g.stride, c0, g.lanes, a.dim);
   const int slot_bytes = ring.slot_bytes();
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
   const int advance = g.lanes * V;
   const uint64_t step = HIDDEN ? step_of(a.drop) : 0;
   const float inv = 1.0f / (float)a.dim;
-  constexpr int S = ring_slots<C>();
+  constexpr int S = ring_slots<T, C, true>();
   const int rows = rows_of(a.rows, g.first, g.stride);
   Ring<T, L, C, S, EDGE> ring_x(ring_memory, 0, a.x, a.ldx, g.first, g.stride, c0, g.lanes, a.dim);
   Ring<T, L, C, S, EDGE> ring_dy(ring_memory, 1, a.dy, a.lddy, g.first, g.stride, c0, g.lanes, a.dim);
@@ -764,7 +769,7 @@ struct NormForward {
   template <int L, int C>
   void operator()(int threads) const {
     auto kernel = norm_forward_kernel<T, L, C, HIDDEN, LAYOUT>;
-    constexpr int per_thread = 16 * C * ring_slots<C>();
+    constexpr int per_thread = 16 * C * ring_slots<T, C, false>();
     static std::atomic<uint64_t> seen{0};
     allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
     static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
@@ -784,7 +789,7 @@ struct NormBackward {
   template <int L, int C>
   void operator()(int threads) const {
     auto kernel = norm_backward_kernel<T, L, C, HIDDEN, LAYOUT>;
-    constexpr int per_thread = std::max(32 * C * ring_slots<C>(), L == 0 ? 0 : C * kVec<T> * 4);
+    constexpr int per_thread = std::max(32 * C * ring_slots<T, C, true>(), L == 0 ? 0 : C * kVec<T> * 4);
     static std::atomic<uint64_t> seen{0};
     allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
     static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
