@@ -31,9 +31,12 @@ enum { kWhole, kEdges, kMoved };
 template <class T, int C>
 constexpr int wide_threads() { return C * kVec<T> <= 16 ? 512 : 256; }
 
-// Blocks of 256 threads per SM that the register allocation aims at: as many as leave nothing spilled.
+// The forward pass runs two blocks of 256 threads per SM and no more: with the rings, 512 threads keep enough in flight, and more of
+// them only mix their reads and writes more finely (2449029x256 fp32: 760 us with two, 834 with three, 956 with one).
+constexpr int kForwardBlocks = 2;
+// Blocks of 256 threads per SM that the register allocation aims at: in the backward pass as many as leave nothing spilled.
 template <class T, int C, bool HIDDEN, bool EDGE>
-constexpr int forward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN && EDGE ? 3 : 4) : C * kVec<T> <= (HIDDEN ? 12 : 16) ? (HIDDEN && EDGE ? 2 : 3) : HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : 2; }
+constexpr int forward_blocks() { return HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : kForwardBlocks; }
 template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 8 : 16) ? 2 : 1; }
 // Slots of the rings.  In the forward pass 32-bit rows do best with little in flight (2 slots of 64 bytes a thread and more: 65536x2048 172 us
@@ -774,7 +777,7 @@ struct NormForward {
     allow_smem(kernel, per_thread * (L == 0 ? wide_threads<T, C>() : 256), seen);
     static const int full = blocks_per_sm(kernel, 256, per_thread * 256);
     constexpr int per = L == 0 ? 1 : 256 / std::max(L, 1);
-    int64_t most = (int64_t)kSMs * (L == 0 ? std::max(1, full * 256 / threads) : full);
+    const int64_t most = (int64_t)kSMs * std::max(1, std::min(full, kForwardBlocks) * 256 / threads);
     int blocks = clamp_blocks((a.rows + per - 1) / per, most);
     if (L == 0) blocks = (blocks + 7) / 8 * 8;
     kernel<<<blocks, threads, per_thread * threads, stream>>>(a);
