@@ -79,13 +79,11 @@ def _laid_like(t, v):
     matrices in the same 16-byte vectors; a copy costs a third of what they lose on rows that lie differently."""
     per = 16 // t.element_size()
     off, step = v.data_ptr() % 16, v.stride(0) % per
-    if t.size(0) <= 1:
-        if t.data_ptr() % 16 == off:
-            return t
-        step = 0
-    elif t.data_ptr() % 16 == off and t.stride(0) % per == step:
+    if t.data_ptr() % 16 == off and (t.stride(0) % per == step or t.size(0) <= 1):
         return t
     rows, width = t.shape
+    if rows <= 1:
+        step = 0
     ld = width + (step - width) % per
     out = t.new_empty(rows * ld + per).as_strided((rows, width), (ld, 1), off // t.element_size())
     return out.copy_(t)
@@ -101,7 +99,7 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _kind(weight, bias, x):
+def _kind(weight, bias):
     """the one type in which both vectors go down: their own, or 32-bit where they differ"""
     if weight is None or bias is None:
         v = bias if weight is None else weight
@@ -140,7 +138,7 @@ def _norm_forward(x, weight, bias, eps, relu, drop, want_stats):
     rows, width = v.shape
     y = _like(x)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
-    kind = _kind(weight, bias, x)
+    kind = _kind(weight, bias)
     w, b = _vector(weight, kind), _vector(bias, kind)
     _call(_native.cuda().rof_layer_norm_forward, x, DTYPES[x.dtype], v.data_ptr(), v.stride(0), rows, width, DTYPES[kind],
           _ptr(w), _ptr(b), eps, relu, _drop_arg(drop, drop[3] if drop else None), y.data_ptr(), width, _ptr(stats))
@@ -149,24 +147,25 @@ def _norm_forward(x, weight, bias, eps, relu, drop, want_stats):
 
 def _norm_backward(ctx, grad):
     v, weight, bias, stats, step = ctx.saved_tensors
-    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    relu, drop = ctx.more
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
     rows, width = v.shape
     dy = _laid_like(_rows(grad), v)
     dx = _like(grad) if need_x else None
-    kind = _kind(weight, bias, v)
+    kind = _kind(weight, bias)
     w, b = _vector(weight, kind), _vector(bias, kind)
-    dw = _like(w) if need_w else None
-    db = _like(b) if need_b else None
+    dw = torch.empty_like(w) if need_w else None
+    db = torch.empty_like(b) if need_b else None
     lib = _native.cuda()
     ws, n = _workspace(lib, rows, width, v) if need_w or need_b else (None, 0)
     _call(lib.rof_layer_norm_backward, v, DTYPES[v.dtype], dy.data_ptr(), dy.stride(0), v.data_ptr(), v.stride(0), rows, width,
-          DTYPES[kind], _ptr(w), _ptr(b), stats.data_ptr(), ctx.relu, _drop_arg(ctx.drop, step), _ptr(dx), width,
-          _ptr(dw), _ptr(db), _ptr(ws), n)
+          DTYPES[kind], _ptr(w), _ptr(b), stats.data_ptr(), relu, _drop_arg(drop, step), _ptr(dx), width, _ptr(dw), _ptr(db),
+          _ptr(ws), n)
     if need_w and dw.dtype is not weight.dtype:
         dw = dw.to(weight.dtype)
     if need_b and db.dtype is not bias.dtype:
         db = db.to(bias.dtype)
-    return dx, dw, db, None, None, None, None
+    return dx, dw, db, None
 
 
 # The wrapper that refuses a second derivative costs 12 us a call: it is only gone through where a graph of the
@@ -181,10 +180,11 @@ def _without_tensor(drop):
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, relu, drop, step):
+    def forward(ctx, x, weight, bias, more):
+        eps, relu, drop = more
         v, y, stats = _norm_forward(x, weight, bias, eps, relu, drop, True)
-        ctx.save_for_backward(v, weight, bias, stats, step)
-        ctx.relu, ctx.drop = relu, _without_tensor(drop)
+        ctx.save_for_backward(v, weight, bias, stats, drop[3] if drop else None)
+        ctx.more = relu, _without_tensor(drop)
         return y
 
     @staticmethod
@@ -209,7 +209,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None
     drop = _check_drop(p, seed, step, row_offset, training, x)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps, bool(relu), drop, drop[3] if drop else None)
+        return _LayerNorm.apply(x, weight, bias, (eps, bool(relu), drop))
     return _norm_forward(x, weight, bias, eps, bool(relu), drop, False)[1]
 
 
@@ -226,21 +226,20 @@ def _dropout_forward(x, bias, relu, drop):
 
 def _dropout_backward(ctx, grad):
     y, step = ctx.saved_tensors
-    need_x, need_b = ctx.needs_input_grad[:2]
+    relu, drop, kind = ctx.more
+    need_x, need_b, _ = ctx.needs_input_grad
     dy = _rows(grad)
     rows, width = dy.shape
     dx = _like(grad) if need_x else None
-    if need_b:
-        dy = _laid_like(dy, dx if dx is not None else y if y is not None else dy)
-    kind = ctx.bias_kind
     lib = _native.cuda()
     db, (ws, n) = None, (None, 0)
     if need_b:
-        db = torch.empty(width, dtype=kind, device=dy.device)
+        dy = _laid_like(dy, _rows(dx) if need_x else _rows(y) if relu else dy)
+        db = dy.new_empty(width, dtype=kind)
         ws, n = _workspace(lib, rows, width, dy)
     _call(lib.rof_dropout_backward, dy, DTYPES[dy.dtype], dy.data_ptr(), dy.stride(0), _ptr(y), width, rows, width, DTYPES[kind],
-          ctx.relu, _drop_arg(ctx.drop, step), _ptr(dx), width, _ptr(db), _ptr(ws), n)
-    return dx, db, None, None, None
+          relu, _drop_arg(drop, step), _ptr(dx), width, _ptr(db), _ptr(ws), n)
+    return dx, db, None
 
 
 _dropout_backward_once = torch.autograd.function.once_differentiable(_dropout_backward)
@@ -248,12 +247,12 @@ _dropout_backward_once = torch.autograd.function.once_differentiable(_dropout_ba
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, bias, relu, drop, step):
+    def forward(ctx, x, bias, more):
+        relu, drop = more
         y = _dropout_forward(x, bias, relu, drop)
         # behind a ReLU the output says which elements were kept and positive
-        ctx.save_for_backward(y if relu else None, step)
-        ctx.relu, ctx.drop = relu, _without_tensor(drop)
-        ctx.bias_kind = bias.dtype if bias is not None else torch.float32
+        ctx.save_for_backward(y if relu else None, drop[3] if drop else None)
+        ctx.more = relu, _without_tensor(drop), bias.dtype if bias is not None else torch.float32
         return y
 
     @staticmethod
@@ -273,7 +272,7 @@ def dropout(x, p=0.0, seed=None, step=0, row_offset=0, training=True, bias=None,
         _check_vector(bias, "bias", x)
     drop = _check_drop(p, seed, step, row_offset, training, x)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        return _Dropout.apply(x, bias, bool(relu), drop, drop[3] if drop else None)
+        return _Dropout.apply(x, bias, (bool(relu), drop))
     return _dropout_forward(x, bias, bool(relu), drop)
 
 
