@@ -8,6 +8,8 @@ repeated by its seed.  `seed` is a number; without one it is drawn from torch's 
 torch.manual_seed and torch.utils.checkpoint control.  `step` is a number or a one-element int64 CUDA tensor that
 is read when the kernel runs: a captured graph that adds to it draws anew on every replay.  The backward pass
 reads the tensor too: change it after the backward pass only (in eager mode autograd refuses a change in between).
+Both passes can be captured into a CUDA graph; as with every torch operation, no eager graph of the same leaves may be
+alive meanwhile (torch ties a leaf's gradient to the stream of the graph that lives).
 
 All sums and statistics are held in 32 bits whatever the matrix's type (float32, bfloat16, float16); results
 are rounded once and are the same bit for bit on every call.  As everywhere in this package there is no CPU path.

@@ -5,7 +5,7 @@ import torch
 import torch.nn.functional as F
 
 import norm_reference as R
-from artifact_b200 import graphs, norm, search
+from artifact_b200 import _native, graphs, norm, search
 from artifact_b200.models import ROF_GCN, ROF_GIN, ROF_inputInfo, SumAggregate
 from artifact_b200.plan import AggregationPlan, empty_padded
 from conftest import load_golden
@@ -62,6 +62,132 @@ def test_layer_norm_many_rows(dtype, rows, dim):
     w, b = randn(dim, seed=3, shift=1.0), randn(dim, seed=4)
     check_norm(x, w, b, dy, what="norm")
     check_norm(x, w, b, calm_gradient(dy, x, w, b, 1e-5), relu=True, p=0.5, seed=3, step=2 ** 40 + 1, row_offset=12345, what="hidden")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [4, 12, 15, 17, 20, 28, 32, 33, 40, 48, 49, 56, 63, 65, 79, 80, 95, 96, 97, 127, 129, 160, 161, 191, 192, 193, 255, 256,
+                                 259, 320, 383, 385, 509, 511, 512, 513, 640, 641, 644, 767, 768, 1023, 1025, 1028, 2047, 2049, 4095, 4097, 8191,
+                                 8193, 8200])
+def test_widths_next_to_every_border(dtype, dim):
+    """the kernels change shape with the width: seven rows each, in both passes, with and without what is fused"""
+    x, dy = randn(7, dim, seed=1, scale=1.5, dtype=dtype), randn(7, dim, seed=2, dtype=dtype)
+    w, b = randn(dim, seed=3, scale=0.3, shift=1.0), randn(dim, seed=4, scale=0.3)
+    check_norm(x, w, b, dy, what="norm")
+    check_norm(x, w, b, calm_gradient(dy, x, w, b, 1e-5), relu=True, p=0.3, seed=12, step=5, what="hidden")
+    check_dropout(x, b, dy, relu=True, p=0.3, seed=12, what="dropout relu")
+    check_dropout(x, b, dy, p=0.3, seed=12, row_offset=1, what="dropout")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, dim", [(100003, 16), (120001, 47), (60000, 50), (30011, 130), (20003, 301), (9001, 501), (12001, 256), (7001, 602),
+                                       (4003, 1024), (2503, 2048), (1203, 4097)])
+def test_many_rows_per_block(dtype, rows, dim):
+    """more rows than one round of the grid takes: rings and tiles go round, the column sums run over many rows"""
+    x, dy = randn(rows, dim, seed=1, dtype=dtype), randn(rows, dim, seed=2, dtype=dtype)
+    w, b = randn(dim, seed=3, scale=0.3, shift=1.0), randn(dim, seed=4, scale=0.3)
+    check_norm(x, w, b, calm_gradient(dy, x, w, b, 1e-5), relu=True, p=0.3, seed=5, what="hidden")
+    check_norm(x, w, b, dy, what="norm")
+    check_dropout(x, b, dy, p=0.3, seed=5, what="dropout")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, dim", [(300, 47), (9001, 50), (77, 130), (64, 301), (700, 602), (33, 1001), (20, 2050), (12, 5001), (9, 9001)])
+def test_padded_rows(dtype, rows, dim):
+    """rows padded to whole vectors, as the framework's own buffers have them, beside contiguous ones"""
+    per = 16 // torch.empty(0, dtype=dtype).element_size()
+
+    def padded(t, more=0):
+        buf = torch.full((rows, -(-dim // per) * per + more), float("nan"), dtype=dtype, device=DEV)
+        buf[:, :dim] = t
+        return buf[:, :dim]
+
+    x, dy = randn(rows, dim, seed=1, dtype=dtype), randn(rows, dim, seed=2, dtype=dtype)
+    w, b = randn(dim, seed=3, scale=0.3, shift=1.0), randn(dim, seed=4, scale=0.3)
+    hidden = dict(relu=True, p=0.3, seed=5, row_offset=2)
+    calm = calm_gradient(dy.clone(), x, w, b, 1e-5)
+    for xs, gs in ((padded(x), padded(dy)), (padded(x), dy), (x, padded(dy)), (padded(x, 3), padded(dy, 8)), (padded(x, per), padded(dy))):
+        check_norm(xs, w, b, gs, what="norm")
+        check_norm(xs, w, b, padded(calm) if gs is not dy else calm, what="hidden", **hidden)
+        check_dropout(xs, b, gs, what="dropout", **hidden)
+        check_dropout(xs, None, gs, what="dropout without bias", p=0.3, seed=5, row_offset=3)
+
+
+def _c_norm(x, w, b, dy, y, dx, relu, drop):
+    """both passes through the C ABI into given outputs -> (dw, db)"""
+    lib, d = _native.cuda(), norm.DTYPES[x.dtype]
+    rows, dim = x.shape
+    stats = torch.full((rows, 2), float("nan"), device=DEV)
+    dw, db = torch.full((dim,), float("nan"), device=DEV), torch.full((dim,), float("nan"), device=DEV)
+    n = lib.rof_layer_norm_workspace_bytes(rows, dim)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)          # whatever was there before
+    s = torch.cuda.current_stream().cuda_stream
+    _native.check(lib.rof_layer_norm_forward(d, x.data_ptr(), x.stride(0), rows, dim, 0, w.data_ptr(), b.data_ptr(), 1e-5, relu, drop,
+                                             y.data_ptr(), y.stride(0), stats.data_ptr(), s))
+    _native.check(lib.rof_layer_norm_backward(d, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), rows, dim, 0, w.data_ptr(),
+                                              b.data_ptr(), stats.data_ptr(), relu, drop, dx.data_ptr(), dx.stride(0), dw.data_ptr(),
+                                              db.data_ptr(), ws.data_ptr(), n, s))
+    return dw, db
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [8, 47, 64, 130, 301, 602, 1001])
+def test_outputs_with_strides_through_the_c_abi(dtype, dim):
+    """every mix of how the four matrices lie; what lies between and behind the rows stays as it was"""
+    rows, w, b = 37, randn(dim, seed=3, scale=0.3, shift=1.0), randn(dim, seed=4, scale=0.3)
+    x0, dy0 = randn(rows, dim, seed=1, dtype=dtype), randn(rows, dim, seed=2, dtype=dtype)
+    calm_gradient(dy0, x0, w, b, 1e-5)
+
+    def laid(t, lead, ld):
+        buf = torch.full((lead + rows * ld + 8,), 7.0, dtype=dtype, device=DEV)
+        view = buf.as_strided((rows, dim), (ld, 1), lead)
+        if t is not None:
+            view.copy_(t)
+        return buf, view
+
+    up = -(-dim // 8) * 8
+    want = R.norm_reference(x0, w, b, relu=True, p=0.3, seed=9, step=3, row_offset=4, dy=dy0)
+    plain = R.dropout_reference(x0, b, True, 0.3, 9, 3, 4, dy=dy0)
+    lib, s = _native.cuda(), torch.cuda.current_stream().cuda_stream
+    drop = _native.Dropout(0.3, 9, 3, None, 4)
+    layouts = ((0, up), (0, dim), (1, dim + 1), (8, up + 8), (3, up))
+    for i, lx in enumerate(layouts):
+        for ly in (layouts[i], layouts[(i + 1) % 5], layouts[(i + 3) % 5]):
+            x, dy = laid(x0, *lx)[1], laid(dy0, *ly)[1]
+            (ybuf, y), (gbuf, dx) = laid(None, *ly), laid(None, *lx)
+            dw, db = _c_norm(x, w, b, dy, y, dx, 1, drop)
+            for got, n in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
+                R.assert_within(got, want[n], f"{lx} {ly} {n}")
+            for buf, view in ((ybuf, y), (gbuf, dx)):
+                view.fill_(7.0)
+                assert (buf == 7.0).all(), (lx, ly)
+            n = lib.rof_layer_norm_workspace_bytes(rows, dim)
+            ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)
+            d = norm.DTYPES[dtype]
+            _native.check(lib.rof_dropout_forward(d, x.data_ptr(), x.stride(0), rows, dim, 0, b.data_ptr(), 1, drop, y.data_ptr(), y.stride(0), s))
+            _native.check(lib.rof_dropout_backward(d, dy.data_ptr(), dy.stride(0), y.data_ptr(), y.stride(0), rows, dim, 0, 1, drop,
+                                                   dx.data_ptr(), dx.stride(0), db.data_ptr(), ws.data_ptr(), n, s))
+            for got, name in ((y, "y"), (dx, "dx"), (db, "db")):
+                R.assert_within(got, plain[name], f"dropout {lx} {ly} {name}")
+            for buf, view in ((ybuf, y), (gbuf, dx)):
+                view.fill_(7.0)
+                assert (buf == 7.0).all(), (lx, ly)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows, dim", [(5, 64), (5, 47), (3, 1001), (40000, 33), (1, 4097)])
+def test_dropout_in_place_through_the_c_abi(dtype, rows, dim):
+    """y may be x itself, and dx dy"""
+    x, dy, b = randn(rows, dim, seed=1, dtype=dtype), randn(rows, dim, seed=2, dtype=dtype), randn(dim, seed=3)
+    lib, d, s = _native.cuda(), norm.DTYPES[dtype], torch.cuda.current_stream().cuda_stream
+    drop = _native.Dropout(0.4, 9, 3, None, 0)
+    for bias in (None, b):
+        want = R.dropout_reference(x, bias, True, 0.4, 9, 3, dy=dy)
+        y, dx = x.clone(), dy.clone()
+        _native.check(lib.rof_dropout_forward(d, y.data_ptr(), dim, rows, dim, 0, norm._ptr(bias), 1, drop, y.data_ptr(), dim, s))
+        _native.check(lib.rof_dropout_backward(d, dx.data_ptr(), dim, y.data_ptr(), dim, rows, dim, 0, 1, drop, dx.data_ptr(), dim, None,
+                                               None, 0, s))
+        R.assert_within(y, want["y"])
+        R.assert_within(dx, want["dx"])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -300,6 +426,33 @@ def test_step_tensor_in_a_captured_graph():
     step.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_capture_beside_a_living_eager_graph():
+    """a step captured while an eager graph of the same tensors waits for its backward pass, which still works afterwards.  The
+    captured one has leaves of its own on them: torch ties a leaf's node to the stream of the graph that lives, and refuses to capture
+    across (for every operation alike)"""
+    x, w, b, dy = randn(300, 100, seed=1), randn(100, seed=2, shift=1.0), randn(100, seed=3), randn(300, 100, seed=4)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def forward(leaves=leaves):
+        return norm.dropout(norm.layer_norm(*leaves, relu=True, p=0.2, seed=1), 0.3, seed=2, bias=leaves[2])
+
+    want = torch.autograd.grad(forward(), leaves, dy)
+    eager = forward()
+    own = [t.detach().requires_grad_(True) for t in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(forward(own), own, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(forward(own), own, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(eager, leaves, dy), want))
 
 
 def test_streams_and_graphs_side_by_side():
