@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(128) norm_backward_columns_plain(const __grid_
 // U vectors that lie `advance` elements apart, e the index of the first.  BACK = false: drop(relu?(x + b)); BACK = true: dy behind the
 // dropout and the ReLU, where with the ReLU the forward's output y says which elements were kept and positive.  DRAW: the
 // generator is asked.
-template <class T, int U, bool BACK, bool DRAW, bool EDGE>
+template <class T, int U, bool BACK, bool DRAW, bool BIAS, bool EDGE>
 __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, int64_t e, int64_t advance, const Pack<T> (&in)[U],
                                              const Pack<T> (&y)[U], const float2 (&b)[kVec<T> / 2], float2 (&o)[U][kVec<T> / 2]) {
   constexpr int V = kVec<T>, H = V / 2;
@@ -476,8 +476,10 @@ __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, i
         for (int t = 0; t < H; ++t) o[u][t] = make_float2(f[t].x <= 0.0f ? 0.0f : o[u][t].x, f[t].y <= 0.0f ? 0.0f : o[u][t].y);
       }
     } else {
+      if constexpr (BIAS) {
 #pragma unroll
-      for (int t = 0; t < H; ++t) o[u][t] = __fadd2_rn(o[u][t], b[t]);
+        for (int t = 0; t < H; ++t) o[u][t] = __fadd2_rn(o[u][t], b[t]);
+      }
       if (a.relu) {
 #pragma unroll
         for (int t = 0; t < H; ++t) o[u][t] = make_float2(relu_of(o[u][t].x), relu_of(o[u][t].y));
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(256, 4) dropout_flat_kernel(const __grid_const
     }
   }
   float2 o[U][V / 2];
-  drop_vectors<T, U, BACK, DRAW, EDGE>(a, step, a.drop.first + i * V, 256 * V, in, yy, zero, o);
+  drop_vectors<T, U, BACK, DRAW, false, EDGE>(a, step, a.drop.first + i * V, 256 * V, in, yy, zero, o);
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (i + u * 256 < vectors) store_vec<T, false>(out + (i + u * 256) * V, 0, V, o[u]);
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(256, 3) dropout_rows_kernel(const __grid_const
         }
       }
       float2 o[U][V / 2];
-      drop_vectors<T, U, BACK, DRAW, EDGE>(a, step, a.drop.first + r * a.dim + c, stride * a.dim, in, yy, b[0], o);
+      drop_vectors<T, U, BACK, DRAW, true, EDGE>(a, step, a.drop.first + r * a.dim + c, stride * a.dim, in, yy, b[0], o);
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + u * stride < a.rows) {
