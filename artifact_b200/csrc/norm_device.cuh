@@ -208,7 +208,7 @@ __device__ __forceinline__ void draw_words(const Drop& d, uint64_t step, int64_t
   if (!EDGE || sh == 0) {
 #pragma unroll
     for (int i = 0; i < C * N / 4; ++i) {
-      const uint4 g = philox7((uint64_t)((e + i / (N / 4) * advance) >> 2) + i % (N / 4), step, d.key);
+      const uint4 g = philox7((uint64_t)(e >> 2) + (i / (N / 4) * (advance >> 2) + i % (N / 4)), step, d.key);
       w[4 * i] = g.x;
       w[4 * i + 1] = g.y;
       w[4 * i + 2] = g.z;

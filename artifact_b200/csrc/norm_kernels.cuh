@@ -5,11 +5,16 @@
 // inside a warp, or the whole block for wide rows); weights, biases and the column sums of the backward
 // pass stay in the thread's registers over all its rows.
 //
-// Rows that do not start on a 16-byte boundary (odd widths in contiguous matrices) use the same vectors: vector i of a row
-// starts at column i * VEC - s, where s is the row start's distance from the boundary below it; the first and last
-// vector are then partial and loaded element by element.  s has period VEC in the row number, and the groups advance by a multiple of
-// VEC rows, so a thread's columns never change.  All matrices of a call must share s (EDGE covers it; without
-// EDGE every vector is whole); calls where they do not run on the *_plain kernels.
+// Rows that do not start on a 16-byte boundary use the same vectors: vector i of a row starts at column i * VEC - s, where s is
+// the row start's distance from the boundary below it; the first and last vector then hold some of their neighbours' elements,
+// which are cleared after the load and not written.  s has period VEC in the row number, and the groups advance by a multiple of
+// VEC rows, so a thread's columns never change.  The inputs of a call must share s; an output that lies differently is
+// written through shared memory.  What is left — inputs that lie differently, rows of more than 8,192 columns — runs on the
+// *_plain kernels.  (Odd widths up to 511 in contiguous matrices: norm_tile.cuh.)
+//
+// Measured on B200, of the measured copy bandwidth (6,460 GB/s; every matrix read or written once per pass): layer norm
+// 2449029x256 fp32 forward 764 us (102 %), back 1,180 us (99 %); 232965x602 fp32 177 us (98 %), 278 us (94 %); 16384x4096
+// bf16 52 us (81 %), 87 us (71 %: a block per row and few warps to cover its two sums).
 #pragma once
 #include "norm_device.cuh"
 
