@@ -1,9 +1,10 @@
-"""ctypes loaders for the two in-tree shared libraries.
+"""Loaders for the in-tree shared libraries: two through ctypes, the torch binding as a module.
 
 There is no fallback of any kind: if a library is missing the loader raises, and every
 product entry point fails with it.
 """
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -12,6 +13,7 @@ from . import build as _build
 _lock = threading.Lock()
 _host = None
 _cuda = None
+_torch_ops = None
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -136,6 +138,24 @@ def cuda():
                 fn.argtypes = args
             _cuda = lib
         return _cuda
+
+
+def torch_ops():
+    """rof_torch.so: layer norm and dropout as torch operations (csrc/torch)."""
+    global _torch_ops
+    if _torch_ops is None:
+        cuda()
+        with _lock:
+            path = _build.torch_lib_path()
+            if not os.path.exists(path):
+                raise NativeLibraryMissing(f"torch binding not built: {path} is missing. Run `python -m artifact_b200.build` "
+                                           "(there is no CPU or eager fallback).")
+            import torch  # noqa: F401  (its libraries have to be loaded first)
+            spec = importlib.util.spec_from_file_location("rof_torch", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _torch_ops = module
+    return _torch_ops
 
 
 class RofError(RuntimeError):

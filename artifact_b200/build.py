@@ -1,17 +1,21 @@
-"""In-tree build of the two native libraries.
+"""In-tree build of the native libraries.
 
 * ``_lib/librof_b200.so`` — CUDA kernels + plan builder + the C ABI declared in
   ``include/rof_b200.h``; compiled by nvcc for sm_100a only.
 * ``_lib/librof_host.so`` — host-only helpers (synthetic graph generators, the
   reuse-group search); compiled by g++ with OpenMP.
+* ``_lib/rof_torch.so`` — autograd nodes of layer norm and dropout over the C ABI
+  (``csrc/torch``); compiled by g++ against the installed torch.
 
-Both are plain shared objects loaded with ctypes; nothing here links against torch.
+The first two are plain shared objects loaded with ctypes and know nothing of torch; the third is a
+Python module that links against the first and against torch.
 Run ``python -m artifact_b200.build`` (or ``__graft_entry__.build()``).
 """
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -61,6 +65,10 @@ def host_lib_path():
     return os.path.join(LIB, "librof_host.so")
 
 
+def torch_lib_path():
+    return os.path.join(LIB, "rof_torch.so")
+
+
 def build_cuda(force=False, verbose=True, ptxas_info=False):
     os.makedirs(LIB, exist_ok=True)
     srcs = [os.path.join(CSRC, s) for s in CUDA_SOURCES if os.path.exists(os.path.join(CSRC, s))]
@@ -89,8 +97,31 @@ def build_host(force=False, verbose=True):
     return target
 
 
+def build_torch(force=False, verbose=True):
+    cuda = build_cuda(verbose=verbose)
+    src = os.path.join(CSRC, "torch", "norm_torch.cpp")
+    target = torch_lib_path()
+    if not force and not _stale(target, [src, os.path.join(INCLUDE, "rof_b200.h"), os.path.abspath(__file__)]):
+        return target
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda_home = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I", INCLUDE]
+    for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+              os.path.join(cuda_home, "include"), sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", target, "-L" + LIB, "-l:" + os.path.basename(cuda), "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(root, "lib"),
+            "-Wl,-rpath," + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
+    _run(cmd, verbose)
+    return target
+
+
 def build_all(force=False, verbose=True):
-    return build_cuda(force, verbose), build_host(force, verbose)
+    """-> the CUDA library and the host library (rof_torch.so is built beside them)"""
+    libs = build_cuda(force, verbose), build_host(force, verbose)
+    build_torch(force, verbose)
+    return libs
 
 
 if __name__ == "__main__":

@@ -13,6 +13,7 @@ from conftest import load_golden
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = {F32: 0, BF16: 1, F16: 2}                     # enum rof_dtype
 
 
 def randn(*shape, seed=0, dtype=F32, scale=1.0, shift=0.0):
@@ -114,7 +115,7 @@ def test_padded_rows(dtype, rows, dim):
 
 def _c_norm(x, w, b, dy, y, dx, relu, drop):
     """both passes through the C ABI into given outputs -> (dw, db)"""
-    lib, d = _native.cuda(), norm.DTYPES[x.dtype]
+    lib, d = _native.cuda(), DTYPES[x.dtype]
     rows, dim = x.shape
     stats = torch.full((rows, 2), float("nan"), device=DEV)
     dw, db = torch.full((dim,), float("nan"), device=DEV), torch.full((dim,), float("nan"), device=DEV)
@@ -162,7 +163,7 @@ def test_outputs_with_strides_through_the_c_abi(dtype, dim):
                 assert (buf == 7.0).all(), (lx, ly)
             n = lib.rof_layer_norm_workspace_bytes(rows, dim)
             ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)
-            d = norm.DTYPES[dtype]
+            d = DTYPES[dtype]
             _native.check(lib.rof_dropout_forward(d, x.data_ptr(), x.stride(0), rows, dim, 0, b.data_ptr(), 1, drop, y.data_ptr(), y.stride(0), s))
             _native.check(lib.rof_dropout_backward(d, dy.data_ptr(), dy.stride(0), y.data_ptr(), y.stride(0), rows, dim, 0, 1, drop,
                                                    dx.data_ptr(), dx.stride(0), db.data_ptr(), ws.data_ptr(), n, s))
@@ -178,12 +179,12 @@ def test_outputs_with_strides_through_the_c_abi(dtype, dim):
 def test_dropout_in_place_through_the_c_abi(dtype, rows, dim):
     """y may be x itself, and dx dy"""
     x, dy, b = randn(rows, dim, seed=1, dtype=dtype), randn(rows, dim, seed=2, dtype=dtype), randn(dim, seed=3)
-    lib, d, s = _native.cuda(), norm.DTYPES[dtype], torch.cuda.current_stream().cuda_stream
+    lib, d, s = _native.cuda(), DTYPES[dtype], torch.cuda.current_stream().cuda_stream
     drop = _native.Dropout(0.4, 9, 3, None, 0)
     for bias in (None, b):
         want = R.dropout_reference(x, bias, True, 0.4, 9, 3, dy=dy)
         y, dx = x.clone(), dy.clone()
-        _native.check(lib.rof_dropout_forward(d, y.data_ptr(), dim, rows, dim, 0, norm._ptr(bias), 1, drop, y.data_ptr(), dim, s))
+        _native.check(lib.rof_dropout_forward(d, y.data_ptr(), dim, rows, dim, 0, bias.data_ptr() if bias is not None else None, 1, drop, y.data_ptr(), dim, s))
         _native.check(lib.rof_dropout_backward(d, dx.data_ptr(), dim, y.data_ptr(), dim, rows, dim, 0, 1, drop, dx.data_ptr(), dim, None,
                                                None, 0, s))
         R.assert_within(y, want["y"])
@@ -305,6 +306,29 @@ def test_layer_norm_extremes():
     check_norm(x, None, None, randn(4, 64, seed=5, dtype=F16), what="large float16")
     # eps = 0 and one column
     check_norm(randn(9, 12, seed=6), None, None, randn(9, 12, seed=7), eps=0.0, what="eps 0")
+
+
+def test_refusals():
+    x, v = torch.zeros(4, 8, device=DEV), torch.zeros(8, device=DEV)
+    for bad in (torch.zeros(7, device=DEV), torch.zeros(1, 8, device=DEV), torch.zeros(8), v.double(), v.half()):
+        with pytest.raises(RuntimeError, match="weight must be"):
+            norm.layer_norm(x, bad)
+        with pytest.raises(RuntimeError, match="bias must be"):
+            norm.layer_norm(x, v, bad)
+        with pytest.raises(RuntimeError, match="bias must be"):
+            norm.dropout(x, bias=bad)
+    norm.layer_norm(x.half(), v.half(), v)                                            # either type beside the other
+    for f in (norm.layer_norm, norm.dropout):
+        with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+            f(x.double())
+        with pytest.raises(RuntimeError, match="at least one dimension"):
+            f(torch.zeros((), device=DEV))
+        for step in (torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int64)):
+            with pytest.raises(RuntimeError, match="step must be"):
+                f(x, p=0.5, seed=1, step=step)
+    for eps in (-1e-9, float("nan")):
+        with pytest.raises(ValueError):
+            norm.layer_norm(x, eps=eps)
 
 
 def test_no_rows_and_no_columns():

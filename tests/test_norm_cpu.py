@@ -63,48 +63,38 @@ def test_no_cpu_path_and_no_other_types():
 @pytest.mark.parametrize("kw", [dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(p=0.5, seed=-1), dict(p=0.5, seed=2 ** 64),
                                 dict(p=0.5, seed=1, step=-1), dict(p=0.5, seed=1, step=2 ** 64), dict(p=0.5, seed=1, row_offset=-1)])
 def test_refused_dropout_arguments(kw):
-    a = dict(p=0.0, seed=None, step=0, row_offset=0) | kw
     with pytest.raises(ValueError):
-        norm._check_drop(a["p"], a["seed"], a["step"], a["row_offset"], True, torch.zeros(2, 2))
+        norm.dropout(torch.zeros(2, 2), **kw)
+    with pytest.raises(ValueError):
+        norm.layer_norm(torch.zeros(2, 2), **kw)
 
 
-def test_step_tensor_is_checked_and_seeds_come_from_torch():
-    x = torch.zeros(2, 2)
-    with pytest.raises(RuntimeError, match="step"):
-        norm._check_drop(0.5, 1, torch.zeros(2, dtype=torch.int64), 0, True, x)
-    with pytest.raises(RuntimeError, match="step"):
-        norm._check_drop(0.5, 1, torch.zeros(1, dtype=torch.int32), 0, True, x)
+def test_generator_arguments_and_seeds_from_torch():
     t = torch.zeros(1, dtype=torch.int64)
-    assert norm._check_drop(0.5, 1, t, 0, True, x) == (0.5, 1, 0, t, 0)
-    assert norm._check_drop(0.5, 1, 0, 0, False, x) is None and norm._check_drop(0.0, 1, 0, 0, True, x) is None
+    assert norm._drop_args(0.5, 1, t, 0, True) == (0.5, 1, 0, 0, t)
+    assert norm._drop_args(0.5, 2 ** 64 - 1, 2 ** 64 - 1, 3, True) == (0.5, 2 ** 64 - 1, 2 ** 64 - 1, 3, None)
+    assert norm._drop_args(0.5, 1, 0, 0, False) == (0.0, 0, 0, 0, None) == norm._drop_args(0.0, None, 0, 0, True)
     torch.manual_seed(5)
     a = [norm.draw_seed() for _ in range(3)]
     torch.manual_seed(5)
     assert a == [norm.draw_seed() for _ in range(3)] and len(set(a)) == 3 and min(a) >= 0
 
 
-def test_vectors_are_checked():
-    x = torch.zeros(4, 8)
-    for v in (torch.zeros(7), torch.zeros(1, 8), torch.zeros(8, dtype=torch.float64), torch.zeros(8, dtype=torch.float16)):
-        with pytest.raises(RuntimeError, match="weight"):
-            norm._check_vector(v, "weight", x)
-    norm._check_vector(torch.zeros(8, dtype=torch.bfloat16), "weight", x.bfloat16())
-    norm._check_vector(torch.zeros(8), "weight", x.bfloat16())
-
-
 def test_rows_views_and_copies():
+    rows_of = _native.torch_ops().rows_of
     x = torch.arange(60.0).view(3, 4, 5)
-    assert norm._rows(x).shape == (12, 5) and norm._rows(x).data_ptr() == x.data_ptr()
-    assert norm._rows(x[0, 0]).shape == (1, 5)
-    assert norm._rows(x.view(12, 5)[:, :3]).stride(0) == 5                           # padded rows stay where they are
-    t = norm._rows(torch.arange(12.0).view(3, 4).t())
+    assert rows_of(x).shape == (12, 5) and rows_of(x).data_ptr() == x.data_ptr()
+    assert rows_of(x[0, 0]).shape == (1, 5)
+    assert rows_of(x.view(12, 5)[:, :3]).stride(0) == 5                           # padded rows stay where they are
+    t = rows_of(torch.arange(12.0).view(3, 4).t())
     assert t.stride() == (3, 1) and torch.equal(t, torch.arange(12.0).view(3, 4).t())
-    assert norm._rows(torch.ones(1, 4).expand(3, 4)).stride() == (4, 1)              # an expanded gradient
-    assert norm._rows(torch.zeros(2, 3, 0)).shape == (6, 0) and norm._rows(torch.zeros(0, 4)).shape == (0, 4)
+    assert rows_of(torch.ones(1, 4).expand(3, 4)).stride() == (4, 1)              # an expanded gradient
+    assert rows_of(torch.zeros(2, 3, 0)).shape == (6, 0) and rows_of(torch.zeros(0, 4)).shape == (0, 4)
 
 
 def test_matrices_are_laid_alike():
     """a gradient whose rows lie differently against the 16-byte boundaries is copied, one that lies alike is not"""
+    laid_like = _native.torch_ops().laid_like
     gen = torch.Generator().manual_seed(1)
     for dtype in (torch.float32, torch.bfloat16):
         per = 16 // torch.empty(0, dtype=dtype).element_size()
@@ -114,13 +104,13 @@ def test_matrices_are_laid_alike():
             for ld in (12, 13, 14, 16, 40):
                 v = flat.as_strided((7, 11), (ld, 1), start + off)
                 for t in (v, v.contiguous(), flat.as_strided((7, 11), (24, 1), start), flat.as_strided((7, 11), (11, 1), start + 1)):
-                    u = norm._laid_like(t, v)
+                    u = laid_like(t, v)
                     assert torch.equal(u, t) and u.stride(1) == 1 and u.stride(0) >= 11
                     for r in range(7):
                         assert (u[r].data_ptr() - v[r].data_ptr()) % 16 == 0
-                assert norm._laid_like(v, v) is v
+                assert laid_like(v, v).data_ptr() == v.data_ptr()
                 one = flat.as_strided((1, 11), (3, 1), start + off)
-                assert (norm._laid_like(flat[start + 2:start + 13].view(1, 11), one).data_ptr() - one.data_ptr()) % 16 == 0
+                assert (laid_like(flat[start + 2:start + 13].view(1, 11), one).data_ptr() - one.data_ptr()) % 16 == 0
 
 
 def test_c_entry_points_refuse_bad_arguments():
