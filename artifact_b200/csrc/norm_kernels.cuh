@@ -728,6 +728,7 @@ bool by_width(int vectors, F&& f) {
     else if (vectors <= 64) f.template operator()<32, 2>(256);
     else if (vectors <= 96) f.template operator()<32, 3>(256);
     else if (vectors <= 128) f.template operator()<32, 4>(256);
+    else if (vectors <= 160) f.template operator()<32, 5>(256);          // (300000x602: 368 us, 445 with a block per row)
     else if (vectors <= 1024) return wide_rows<T, 2>(vectors, f);
     else return wide_rows<T, 4>(vectors, f);
   } else if constexpr (PASS == kBackwardHidden) {
