@@ -39,9 +39,11 @@ constexpr int wide_threads() { return C * kVec<T> <= 16 ? 512 : 256; }
 // The forward pass runs two blocks of 256 threads per SM and no more: with the rings, 512 threads keep enough in flight, and more of
 // them only mix their reads and writes more finely (2449029x256 fp32: 760 us with two, 834 with three, 956 with one).
 constexpr int kForwardBlocks = 2;
-// Blocks of 256 threads per SM that the register allocation aims at: in the backward pass as many as leave nothing spilled.
+// Blocks of 256 threads per SM that the register allocation aims at: in the backward pass as many as leave nothing spilled; in the
+// forward pass two, where 32 elements a thread with the generator and partial vectors would spill 400 bytes one (200000x1001
+// fp32: 351 us, 433 with two; 20 elements, 300000x602: 264 us with two, 357 with one).
 template <class T, int C, bool HIDDEN, bool EDGE>
-constexpr int forward_blocks() { return HIDDEN && EDGE && C * kVec<T> > 16 ? 1 : kForwardBlocks; }
+constexpr int forward_blocks() { return HIDDEN && EDGE && C * kVec<T> > 24 ? 1 : kForwardBlocks; }
 template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 8 : 16) ? 2 : 1; }
 // Slots of the rings.  In the forward pass 32-bit rows do best with little in flight (2 slots of 64 bytes a thread and more: 65536x2048 172 us
