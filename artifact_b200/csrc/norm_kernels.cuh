@@ -543,11 +543,19 @@ __global__ void __launch_bounds__(256, 4) dropout_flat_kernel(const __grid_const
   }
 }
 
+// Rows that a thread of dropout_rows_kernel takes at once, and blocks per SM that its registers aim at.  With the generator, sixteen
+// elements; behind a ReLU the backward pass only streams, and whole 32-bit vectors do it with many warps (232965x256:
+// 124 us, 133 with four rows and four blocks), 16-bit ones with many rows (1000000x64 bf16: 73 us, 86).
+template <class T, bool STREAM, bool EDGE>
+constexpr int drop_rows_at_once() { return !STREAM ? 16 / kVec<T> : sizeof(T) == 2 ? 8 : EDGE ? 4 : 2; }
+template <class T, bool STREAM, bool EDGE>
+constexpr int drop_row_blocks() { return !STREAM ? 3 : sizeof(T) == 2 ? 2 : EDGE ? 3 : 6; }
+
 // Thread = vector `c` of the rows first, first + stride, ...; a.lanes threads side by side cover a tile of a row.  U rows at a time:
 // their loads and their calls of the generator run side by side.
 template <class T, bool BACK, bool DRAW, bool EDGE>
-__global__ void __launch_bounds__(256, 3) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
-  constexpr int V = kVec<T>, U = BACK && !DRAW ? 4 : 16 / V;
+__global__ void __launch_bounds__(256, drop_row_blocks<T, BACK && !DRAW, EDGE>()) dropout_rows_kernel(const __grid_constant__ DropArgs a) {
+  constexpr int V = kVec<T>, U = drop_rows_at_once<T, BACK && !DRAW, EDGE>();
   extern __shared__ float columns[];
   const int groups = blockDim.x / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes;
   const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
