@@ -938,6 +938,11 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
     else if (l.edge) blocks = launch_dropout_rows<T, BACK, false, true>(a, groups, threads, tiles, smem, stream);
     else blocks = launch_dropout_rows<T, BACK, false, false>(a, groups, threads, tiles, smem, stream);
   } else {
+    // the sums first: dx may be dy itself
+    if (BACK && a.partial != nullptr) {
+      blocks = clamp_blocks((a.rows + 31) / 32, column_blocks_cap(a.rows, a.dim));
+      dropout_columns_plain<T><<<dim3((a.dim + 127) / 128, blocks), 128, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);
+    }
     if (a.out != nullptr) {
       // contiguous, and element i0 of a group lies at a multiple of four elements
       const auto fours = [&](const void* p, int64_t ld) {
@@ -946,10 +951,6 @@ cudaError_t launch_dropout(const DropArgs& given, cudaStream_t stream) {
       const int even = (fours(a.x, a.ldx) ? 1 : 0) | (fours(a.y, a.ldy) ? 2 : 0) | (fours(a.out, a.ldo) ? 4 : 0);
       const int64_t groups = a.rows * a.dim / 4 + 2;
       dropout_any_kernel<T, BACK><<<(int)((groups + 511) / 512), 256, 0, stream>>>(a, even);
-    }
-    if (BACK && a.partial != nullptr) {
-      blocks = clamp_blocks((a.rows + 31) / 32, column_blocks_cap(a.rows, a.dim));
-      dropout_columns_plain<T><<<dim3((a.dim + 127) / 128, blocks), 128, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);
     }
   }
   if (!BACK || a.partial == nullptr) return cudaGetLastError();

@@ -1,0 +1,55 @@
+"""Layer norm and dropout on the GPU at calls that the other tests do not make."""
+import pytest
+import torch
+
+import norm_reference as R
+from artifact_b200 import _native
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = {F32: 0, BF16: 1, F16: 2}                     # enum rof_dtype
+
+
+def randn(*shape, seed=0, dtype=F32, scale=1.0, shift=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * scale + shift).to(dtype).to(DEV)
+
+
+def padded(t, ld):
+    """t with rows `ld` elements apart"""
+    buf = torch.full((t.size(0), ld), 7.0, dtype=t.dtype, device=DEV)
+    view = buf[:, :t.size(1)]
+    view.copy_(t)
+    return view
+
+
+def c_dropout(x, bias, dy, y, dx, relu, drop):
+    """both passes of rof_dropout_* into the given outputs -> dbias"""
+    lib, d, s = _native.cuda(), DTYPES[x.dtype], torch.cuda.current_stream().cuda_stream
+    rows, dim = x.shape
+    vt = DTYPES[bias.dtype]
+    db = torch.full((dim,), float("nan"), dtype=bias.dtype, device=DEV)
+    n = lib.rof_layer_norm_workspace_bytes(rows, dim)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)          # whatever was there before
+    _native.check(lib.rof_dropout_forward(d, x.data_ptr(), x.stride(0), rows, dim, vt, bias.data_ptr(), relu, drop, y.data_ptr(), y.stride(0), s))
+    _native.check(lib.rof_dropout_backward(d, dy.data_ptr(), dy.stride(0), y.data_ptr() if relu else None, y.stride(0), rows, dim, vt, relu, drop,
+                                           dx.data_ptr(), dx.stride(0), db.data_ptr(), ws.data_ptr(), n, s))
+    return db
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("relu", [0, 1])
+@pytest.mark.parametrize("rows, dim", [(1, 8), (5, 64), (70, 47), (9001, 47), (33, 602), (3, 1001)])
+def test_dropout_gradients_in_place_with_a_bias_gradient(dtype, relu, rows, dim):
+    """dx may be dy itself, on every path: dbias is the sum of what dy was"""
+    x, b = randn(rows, dim, seed=1, dtype=dtype), randn(dim, seed=3)
+    dy0 = randn(rows, dim, seed=2, dtype=dtype)
+    want = R.dropout_reference(x, b, bool(relu), 0.4, 9, 3, dy=dy0)
+    # y like dy, padded to whole vectors, and off by one element
+    for ld in (dim, -(-dim // 8) * 8, dim + 1):
+        dy = dy0.clone()
+        y = padded(torch.zeros_like(x), ld)
+        db = c_dropout(x, b, dy, y, dy, relu, _native.Dropout(0.4, 9, 3, None, 0))
+        for got, name in ((y, "y"), (dy, "dx"), (db, "db")):
+            R.assert_within(got, want[name], f"ld {ld} {name}")
