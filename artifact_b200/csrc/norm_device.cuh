@@ -252,6 +252,21 @@ __device__ __forceinline__ float relu_of(float z) {
   return z;
 }
 
+// Behind a ReLU a dropout's backward pass asks the output which elements were kept and positive.  With a 32-bit bias a sum may be positive
+// and still round to a zero of a 16-bit type: half of the type's smallest value and less.  That zero is stored with its sign set; every
+// other zero is +0 (the ReLU and the dropout make no other).
+template <class T> constexpr float kRoundsToZero = 0.0f;
+template <> constexpr float kRoundsToZero<__nv_bfloat16> = 0x1p-134f;
+template <> constexpr float kRoundsToZero<__half> = 0x1p-25f;
+template <class T>
+__device__ __forceinline__ float marked(float z) { return z > 0.0f && z <= kRoundsToZero<T> ? -0.0f : z; }
+template <class T>
+__device__ __forceinline__ bool passed(T y) {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(y) != 0;
+  else return *reinterpret_cast<const uint16_t*>(&y) != 0;
+}
+__device__ __forceinline__ float passed_of(float y, float v) { return __float_as_uint(y) != 0 ? v : 0.0f; }
+
 __device__ __forceinline__ float affine(float h, float w, float b) { return __fmaf_rn(h, w, b); }
 
 template <class T>

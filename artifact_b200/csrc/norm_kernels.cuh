@@ -480,7 +480,7 @@ __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, i
         float2 f[H];
         unpack<T>(y[u], f);
 #pragma unroll
-        for (int t = 0; t < H; ++t) o[u][t] = make_float2(f[t].x <= 0.0f ? 0.0f : o[u][t].x, f[t].y <= 0.0f ? 0.0f : o[u][t].y);
+        for (int t = 0; t < H; ++t) o[u][t] = make_float2(passed_of(f[t].x, o[u][t].x), passed_of(f[t].y, o[u][t].y));
       }
     } else {
       if constexpr (BIAS) {
@@ -494,6 +494,14 @@ __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, i
     }
   }
   scale_elements(o, a.drop.scale);
+  if constexpr (!BACK && BIAS && sizeof(T) == 2) {
+    if (a.relu && a.bf32) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < H; ++t) o[u][t] = make_float2(marked<T>(o[u][t].x), marked<T>(o[u][t].y));
+    }
+  }
   if constexpr (DRAW) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -538,7 +546,7 @@ __global__ void __launch_bounds__(256, 4) dropout_flat_kernel(const __grid_const
     float z = to_float(x[e]);
     const bool keep = !DRAW || kept(a.drop, step, a.drop.first + e);
     if (!BACK && a.relu) z = relu_of(z);
-    if (two && to_float(y[e]) <= 0.0f) z = 0.0f;
+    if (two && !passed(y[e])) z = 0.0f;
     out[e] = from_float<T>(keep ? z * a.drop.scale : 0.0f);
   }
 }
@@ -649,12 +657,13 @@ __global__ void __launch_bounds__(256, 4) dropout_any_kernel(const __grid_consta
       if (two && !(full && (whole & 2))) y[t] = reinterpret_cast<const T*>(a.y)[r * a.ldy + c];
       float z = to_float(in[t]);
       if constexpr (BACK) {
-        if (two && to_float(y[t]) <= 0.0f) z = 0.0f;
+        if (two && !passed(y[t])) z = 0.0f;
       } else {
         if (a.bias != nullptr) z += vector_at<T>(a.bias, a.bf32, c);
         if (a.relu) z = relu_of(z);
       }
       z *= a.drop.scale;
+      if (!BACK && a.relu) z = marked<T>(z);
       out[t] = from_float<T>(draw && words[t] <= a.drop.last ? 0.0f : z);
       if (!(full && (whole & 4))) reinterpret_cast<T*>(a.out)[r * a.ldo + c] = out[t];
       if (++c == a.dim) {
@@ -674,7 +683,7 @@ __global__ void __launch_bounds__(128) dropout_columns_plain(const __grid_consta
   const int64_t r0 = (int64_t)blockIdx.y * run_rows, r1 = min(a.rows, r0 + run_rows);
   float sum = 0.0f;
   for (int64_t r = r0; r < r1; ++r) {
-    const bool keep = a.relu ? !(to_float(reinterpret_cast<const T*>(a.y)[r * a.ldy + c]) <= 0.0f)
+    const bool keep = a.relu ? passed(reinterpret_cast<const T*>(a.y)[r * a.ldy + c])
                              : !a.drop.on || kept(a.drop, step, a.drop.first + r * a.dim + c);
     if (keep) sum += to_float(reinterpret_cast<const T*>(a.x)[r * a.ldx + c]) * a.drop.scale;
   }

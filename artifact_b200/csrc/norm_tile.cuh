@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
             float2 y[P];
             read(pb, y);
 #pragma unroll
-            for (int j = 0; j < P; ++j) v[j] = make_float2(y[j].x <= 0.0f ? 0.0f : v[j].x, y[j].y <= 0.0f ? 0.0f : v[j].y);
+            for (int j = 0; j < P; ++j) v[j] = make_float2(passed_of(y[j].x, v[j].x), passed_of(y[j].y, v[j].y));
           }
         } else {
 #pragma unroll
@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
         for (int j = 0; j < P; ++j) {
           v[j] = __fmul2_rn(v[j], both(a.drop.scale));
           if constexpr (kBack) ab[j] = __fadd2_rn(ab[j], v[j]);
+          if (!kBack && sizeof(T) == 2 && a.relu && a.f32) v[j] = make_float2(marked<T>(v[j].x), marked<T>(v[j].y));
           write(pa, j, v[j]);
         }
       }

@@ -215,7 +215,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
                         int64_t first_row, const MaybeTensor& step_tensor) {
     const Tensor t = step_tensor.value_or(Tensor());
     const Tensor y = dropout_forward(x, bias.value_or(Tensor()), relu, Drop{p, seed, step, first_row}, t);
-    // behind a ReLU the output says which elements were kept and positive
+    // behind a ReLU the output's bits say which elements were kept and positive
     ctx->save_for_backward({relu ? y : Tensor(), t});
     ctx->saved_data["drop"] = std::vector<int64_t>{seed, step, first_row, relu, bias.has_value(),
                                                    bias.has_value() && bias->scalar_type() == at::kFloat};

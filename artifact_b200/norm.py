@@ -59,7 +59,8 @@ def dropout(x, p=0.0, seed=None, step=0, row_offset=0, training=True, bias=None,
     x: a CUDA tensor [..., width] of float32, bfloat16 or float16 with any strides; bias: a vector of `width` entries,
     float32 or of x's type, or None.  Each element is zeroed with probability p and scaled by 1 / (1 - p) otherwise, only where
     `training`; p = 1 zeroes everything.  The choice depends on (seed, step, element index) alone, the index counted from
-    row `row_offset` of the whole matrix.  Returns a contiguous tensor like x."""
+    row `row_offset` of the whole matrix.  Returns a contiguous tensor like x.  Behind the ReLU a positive sum that rounds to zero
+    (16-bit x beside a float32 bias) is returned as -0: its gradient is not zero, and the backward pass reads that from the output."""
     return _native.torch_ops().dropout(x, bias, bool(relu), *_drop_args(p, seed, step, row_offset, training))
 
 

@@ -348,14 +348,16 @@ int rof_layer_norm_backward(int dtype, const void* dy, int64_t lddy, const void*
 
 /*
  * y = drop(relu?(x + bias)): dropout, with the bias add and the activation that stand before it in a GCN stack
- * (reuse_conv.py:150, ROF_main.py:181).  bias and drop may be NULL.  y may be x itself.
+ * (reuse_conv.py:150, ROF_main.py:181).  bias and drop may be NULL.  y may be x itself.  With relu, an element that is kept and
+ * positive and rounds to zero (16-bit types beside a 32-bit bias) is stored as -0, and every other zero as +0.
  */
 int rof_dropout_forward(int dtype, const void* x, int64_t ldx, int64_t rows, int dim, int vdtype, const void* bias, int relu,
                         const rof_dropout* drop, void* y, int64_t ldy, void* stream);
 
 /*
  * Gradients of the call above: dx and dbias = sum over the rows of dx before its rounding; either may be NULL.  With relu, `y` is the forward's
- * output, which says by itself which elements were kept and positive; without, it is not read and may be NULL.  dx may be dy itself.
+ * output, whose bits say which elements were kept and positive (all but +0); without, it is not read and may be NULL.  dx may be dy
+ * itself.
  * workspace as above (rof_layer_norm_workspace_bytes), needed where dbias is given.
  */
 int rof_dropout_backward(int dtype, const void* dy, int64_t lddy, const void* y, int64_t ldy, int64_t rows, int dim, int vdtype,

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import norm_reference as R
-from artifact_b200 import _native
+from artifact_b200 import _native, norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -53,3 +53,41 @@ def test_dropout_gradients_in_place_with_a_bias_gradient(dtype, relu, rows, dim)
         db = c_dropout(x, b, dy, y, dy, relu, _native.Dropout(0.4, 9, 3, None, 0))
         for got, name in ((y, "y"), (dy, "dx"), (db, "db")):
             R.assert_within(got, want[name], f"ld {ld} {name}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("dim", [8, 47, 64, 100, 301, 602, 2049, 4097])
+def test_relu_gradients_where_the_output_rounds_to_zero(dtype, p, dim):
+    """x + bias may lie between zero and the type's smallest value: the output is zero, its gradient is not"""
+    rows = 37
+    least = 2.0 ** (-24 if dtype == F16 else -133)                     # the type's smallest value
+    x = torch.zeros(rows, dim, dtype=dtype, device=DEV)
+    x[::3] = least
+    x[2::6] = -0.0
+    x[1::6] = randn(len(range(1, rows, 6)), dim, seed=1, dtype=dtype)
+    sizes = torch.tensor([0.25, 0.5, 0.49, 0.51, -0.5, 1.5, 0.0, -0.75, 1.0 / 256])
+    b = (sizes[torch.arange(dim) % 9].double() * least).float().to(DEV)
+    dy = randn(rows, dim, seed=2, dtype=dtype)
+    drop = dict(p=p, seed=5, step=2) if p else {}
+    want = R.dropout_reference(x, b, True, dy=dy, **drop)
+    zeros = (want["dx"][0] != 0).sum()
+    assert zeros > 0.3 * (1 - p) * rows * dim
+    per = 8
+    wide = -(-dim // per) * per + per
+    for xs, gs in ((x, dy), (padded(x, wide), dy), (x, padded(dy, wide)), (padded(x, dim + 1), padded(dy, dim + 2))):
+        leaf, bias = xs.detach().requires_grad_(True), b.clone().requires_grad_(True)
+        y = norm.dropout(leaf, bias=bias, relu=True, **drop)
+        R.assert_within(y, want["y"], "y")
+        assert (want["y"][0][torch.signbit(y).cpu().numpy()] > 0).all()     # no other zero has a sign
+        only, = torch.autograd.grad(y, leaf, gs, retain_graph=True)
+        gx, gb = torch.autograd.grad(y, (leaf, bias), gs)
+        R.assert_within(only, want["dx"], "dx alone")
+        R.assert_within(gx, want["dx"], "dx")
+        R.assert_within(gb, want["db"], "db")
+    # the column sums of matrices that lie differently
+    for ldy in (dim, wide, dim + 1):
+        y, dx = padded(torch.zeros_like(x), ldy), torch.empty_like(dy)
+        db = c_dropout(x, b, dy, y, dx, 1, _native.Dropout(p, 5, 2, None, 0) if p else None)
+        for got, name in ((y, "y"), (dx, "dx"), (db, "db")):
+            R.assert_within(got, want[name], f"ld {ldy} {name}")
