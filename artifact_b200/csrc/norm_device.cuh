@@ -165,10 +165,17 @@ struct Ring {
   }
 };
 
-// 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place
+// 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place; of zero and infinity the approximation is the value,
+// and the step would make a NaN of it
 __device__ __forceinline__ float rsqrt_of(float v) {
   const float r = rsqrtf(v);
-  return __fmaf_rn(0.5f * r, __fmaf_rn(-(v * r), r, 1.0f), r);
+  return v > 0.0f && v < INFINITY ? __fmaf_rn(0.5f * r, __fmaf_rn(-(v * r), r, 1.0f), r) : r;
+}
+
+// The variance from a row's mean square deviation from a first mean that is `off` from the mean.  Where the squares pass the range of
+// 32 bits it is infinite: the row then has rstd 0 and becomes its bias.
+__device__ __forceinline__ float variance_of(float square, float off) {
+  return square < INFINITY ? fmaxf(__fmaf_rn(-off, off, square), 0.0f) : square;
 }
 
 // Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.

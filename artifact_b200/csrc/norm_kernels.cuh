@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
     const float off = dev.x * inv;
     mean += off;
     minus = both(-mean);
-    const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    const float rstd = rsqrt_of(variance_of(dev.y * inv, off) + a.eps);
     if (stats != nullptr) {
       if (g.lane == 0) *stats = make_float2(mean, rstd);
       stats += g.stride;
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(256) norm_forward_plain(const __grid_constant_
     dev = g.sum(dev, buf[1]);
     const float off = dev.x * inv;
     mean += off;
-    const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+    const float rstd = rsqrt_of(variance_of(dev.y * inv, off) + a.eps);
     if (a.stats != nullptr && g.lane == 0) a.stats[r] = make_float2(mean, rstd);
     for (int c = g.lane; c < a.dim; c += g.lanes) {
       float z = affine((to_float(x[c]) - mean) * rstd, a.weight != nullptr ? vector_at<T>(a.weight, a.wf32, c) : 1.0f,

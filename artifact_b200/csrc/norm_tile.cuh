@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
         const float off = dev.x * inv;
         mean += off;
         minus = both(-mean);
-        const float rstd = rsqrt_of(fmaxf(__fmaf_rn(-off, off, dev.y * inv), 0.0f) + a.eps);
+        const float rstd = rsqrt_of(variance_of(dev.y * inv, off) + a.eps);
         if (a.stats != nullptr && g.lane == 0) *stats = make_float2(mean, rstd);
 #pragma unroll
         for (int j = 0; j < P; ++j) {

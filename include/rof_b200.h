@@ -328,7 +328,8 @@ typedef struct rof_dropout {
 /*
  * y = drop(relu?((x - mean) * rstd * weight + bias)) for every row, mean and rstd = 1 / sqrt(variance + eps) over its
  * `dim` columns.  weight (1), bias (0) and drop (nothing dropped) may be NULL.  stats: [rows][2], the rows' mean and rstd for the
- * backward call; may be NULL.  y must not overlap x.
+ * backward call; may be NULL.  y must not overlap x.  Where a row's variance passes the range of 32 bits, rstd is 0: the row becomes its
+ * bias, its dx is zero.  Where sums of its values do, it turns to NaN, as it does where a value is infinite or NaN.
  */
 int rof_layer_norm_forward(int dtype, const void* x, int64_t ldx, int64_t rows, int dim, int vdtype, const void* weight,
                            const void* bias, float eps, int relu, const rof_dropout* drop, void* y, int64_t ldy,

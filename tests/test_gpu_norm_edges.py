@@ -1,6 +1,8 @@
 """Layer norm and dropout on the GPU at calls that the other tests do not make."""
+import numpy as np
 import pytest
 import torch
+import torch.nn.functional as F
 
 import norm_reference as R
 from artifact_b200 import _native, norm
@@ -91,3 +93,32 @@ def test_relu_gradients_where_the_output_rounds_to_zero(dtype, p, dim):
         db = c_dropout(x, b, dy, y, dx, 1, _native.Dropout(p, 5, 2, None, 0) if p else None)
         for got, name in ((y, "y"), (dx, "dx"), (db, "db")):
             R.assert_within(got, want[name], f"ld {ldy} {name}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [8, 47, 64, 130, 602, 2048, 9000])
+def test_rows_whose_variance_passes_the_range_of_32_bits(dtype, dim):
+    """1 / sqrt(infinity) is zero: such a row is its bias, and its gradient is zero; the other rows do not notice"""
+    x = randn(7, dim, seed=1, dtype=dtype)
+    w, b = randn(dim, seed=3, shift=1.0), randn(dim, seed=4)
+    dy = randn(7, dim, seed=2, dtype=dtype)
+    big = torch.where(torch.arange(dim, device=DEV) % 2 == 0, 3e19, -1e20)
+    x2 = x.clone()
+    x2[1], x2[5] = big.to(dtype), (big * 1e10).to(dtype)
+    rows = [0, 2, 3, 4, 6]
+    leaves, others = [t.clone().requires_grad_(True) for t in (x2, w, b)], [t.clone().requires_grad_(True) for t in (x[rows], w, b)]
+    y, small = norm.layer_norm(*leaves), norm.layer_norm(*others)
+    assert torch.equal(y[1].float(), b.to(dtype).float()) and torch.equal(y[5].float(), b.to(dtype).float())
+    want = R.norm_reference(x[rows], w, b, dy=dy[rows])
+    gx, gw, gb = torch.autograd.grad(y, leaves, dy)
+    R.assert_within(y[rows], want["y"], "y")
+    R.assert_within(gx[rows], want["dx"], "dx")
+    assert (gx[[1, 5]] == 0).all()
+    R.assert_within(gw, want["dw"], "dw")                              # h is zero in those rows
+    total = dy.double().sum(0).cpu().numpy()
+    assert (np.abs(gb.double().cpu().numpy() - total) <= 16 * R.U * dy.double().abs().sum(0).cpu().numpy()).all()
+    for p in (0.0, 0.5):
+        hidden = norm.layer_norm(x2, w, b, relu=True, p=p, seed=3)
+        keep = torch.from_numpy(R.keep_mask(7, dim, p, 3)).to(DEV)
+        assert torch.equal(hidden[[1, 5]], torch.where(keep, F.relu(b).expand(7, dim) / (1 - p), 0.0).to(dtype)[[1, 5]])
+    assert torch.equal(norm.layer_norm(x, w, b, eps=float("inf")), b.to(dtype).expand(7, dim))
