@@ -112,14 +112,17 @@ class ROF_GCN(torch.nn.Module):
     def forward(self, features, inputInfo, edge_index=None, seed=None, step=0, row_offset=0):
         h = features
         last = len(self.layers) - 1
-        if not torch.is_grad_enabled() and self.activation is F.relu:
+        counter = self.dropout_source == "counter"
+        # in training mode a pass without gradients drops too (a reentrant checkpoint's first pass is one); a stack without norm and
+        # counter has always taken the pass of inference there, and keeps it
+        due = self.training and self.dropout > 0 and (counter or self.norms is not None)
+        if not torch.is_grad_enabled() and self.activation is F.relu and not due:
             # inference: bias and ReLU are fused into the store of the gather kernel (with a norm, the ReLU follows that)
             for i, layer in enumerate(self.layers):
                 h = layer.forward_fused(h, inputInfo, relu=i < last and self.norms is None)
                 if i < last and self.norms is not None:
                     h = self._between(h, i, None, None)
             return h
-        counter = self.dropout_source == "counter"
         if counter and seed is None and self.training and self.dropout > 0:
             seed = N.draw_seed()
         for i, layer in enumerate(self.layers):

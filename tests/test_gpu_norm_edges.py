@@ -5,7 +5,8 @@ import torch
 import torch.nn.functional as F
 
 import norm_reference as R
-from artifact_b200 import _native, norm
+from artifact_b200 import _native, graphs, norm, search
+from artifact_b200.models import ROF_GCN, ROF_inputInfo
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -122,3 +123,50 @@ def test_rows_whose_variance_passes_the_range_of_32_bits(dtype, dim):
         keep = torch.from_numpy(R.keep_mask(7, dim, p, 3)).to(DEV)
         assert torch.equal(hidden[[1, 5]], torch.where(keep, F.relu(b).expand(7, dim) / (1 - p), 0.0).to(dtype)[[1, 5]])
     assert torch.equal(norm.layer_norm(x, w, b, eps=float("inf")), b.to(dtype).expand(7, dim))
+
+
+# ---- in the models --------------------------------------------------------------------------------
+def gcn(norm_kind="layer", source="counter", dropout=0.4, activation=F.relu, layers=2):
+    g = graphs.config1()
+    info = ROF_inputInfo.from_layouts(g.indptr_dst, search.search_graph(g, 3), device=DEV)
+    torch.manual_seed(0)
+    model = ROF_GCN(40, 16, 7, layers, activation=activation, dropout=dropout, add_self_loops=False, reuse_size=info.reuse_size,
+                    norm=norm_kind, dropout_source=source).to(DEV)
+    return model, info, randn(g.num_nodes, 40, seed=1)
+
+
+@pytest.mark.parametrize("norm_kind, source", [(None, "counter"), ("layer", "counter"), ("layer", "torch")])
+def test_training_mode_without_gradients_drops_too(norm_kind, source):
+    """a pass in training mode is the same with and without gradients (the first pass of a reentrant checkpoint is one without)"""
+    model, info, x = gcn(norm_kind, source)
+
+    def run():
+        torch.manual_seed(3)
+        return model(x, info, seed=11, step=4)
+
+    want = run()
+    with torch.no_grad():
+        assert torch.equal(run(), want)
+    x.requires_grad_(True)
+    params = [p for p in model.parameters() if p.requires_grad and p.shape[0] != info.reuse_size]
+    torch.manual_seed(3)
+    out = torch.utils.checkpoint.checkpoint(lambda t: model(t, info, seed=11, step=4), x, use_reentrant=True)
+    assert torch.equal(out, want)
+    grads = torch.autograd.grad(run().square().sum(), params)
+    for p in params:
+        p.grad = None
+    out.square().sum().backward()
+    for p, g in zip(params, grads):
+        assert torch.equal(p.grad, g)
+    model.eval()
+    with torch.no_grad():
+        got = model(x, info)
+    assert (got - model(x, info)).abs().max() <= 2e-5 * got.abs().max()
+
+
+def test_the_plain_stack_keeps_its_pass_without_gradients():
+    """upstream's stack under no_grad is the fused inference pass, whatever its mode"""
+    model, info, x = gcn(None, "torch")
+    with torch.no_grad():
+        got = model(x, info)
+        assert torch.equal(got, model.eval()(x, info))
