@@ -5,6 +5,7 @@ the call sites (ROF_main.py:164-174, 192-200, 230; ROF_evaluation/cuda/middle-ro
 import numpy as np
 import torch
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import norm as N
 from .plan import AggregationPlan, scale_rows
@@ -74,6 +75,21 @@ class ROF_inputInfo:
         return f"ROF_inputInfo(partSize={self.partSize}, warpPerBlock={self.warpPerBlock}, " + ", ".join(parts) + ")"
 
 
+def _stands_alone(module, kind):
+    """whether a call of `module` is `kind`'s forward and nothing else, so that a pass fused with it may take its place: no other class,
+    no hooks"""
+    return (getattr(module.forward, "__func__", None) is kind.forward and not module._forward_hooks and not module._forward_pre_hooks
+            and not module._backward_hooks and not module._backward_pre_hooks and not _has_any_global_hook())
+
+
+def _norm_relu_dropout(m, h, relu, drop):
+    """dropout(relu?(m(h))) -> (its value, whether the ReLU and the dropout are in it): one pass where `m` is a LayerNorm of norm.py that
+    stands alone, else the call of the module"""
+    if _stands_alone(m, N.LayerNorm) and not m.relu and m.p == 0:
+        return N.layer_norm(h, m.weight, m.bias, m.eps, relu=relu, **drop), True
+    return m(h), False
+
+
 class ROF_GCN(torch.nn.Module):
     """n_layers hidden ROF_GCNConv layers + one output layer; activation and dropout between
     layers (constructor keywords of ROF_main.py:192-200).  Two keywords upstream does not have:
@@ -97,17 +113,14 @@ class ROF_GCN(torch.nn.Module):
     def _between(self, h, i, bias, drop):
         """what stands between layer i and the next: norm, activation, dropout (`drop`: its keywords, or None)"""
         relu = self.activation is F.relu
-        fused = drop if relu and drop is not None else {}
         if self.norms is not None:
-            m = self.norms[i]
-            h = N.layer_norm(h, m.weight, m.bias, m.eps, relu=relu, **fused)
-        elif relu:
-            h = N.dropout(h, bias=bias, relu=True, **fused)
-        if not relu:
-            h = self.activation(h)
-            if drop is not None:
-                h = N.dropout(h, **drop)
-        return h
+            h, done = _norm_relu_dropout(self.norms[i], h, relu, drop if relu and drop is not None else {})
+            if done and relu:
+                return h
+        if relu and drop is not None:
+            return N.dropout(h, bias=bias, relu=True, **drop)
+        h = self.activation(h)
+        return h if drop is None else N.dropout(h, **drop)
 
     def forward(self, features, inputInfo, edge_index=None, seed=None, step=0, row_offset=0):
         h = features
@@ -129,7 +142,7 @@ class ROF_GCN(torch.nn.Module):
             if i and not counter:
                 h = F.dropout(h, self.dropout, self.training)
             # the fused pass adds the bias itself
-            bare = i < last and counter and self.norms is None and self.activation is F.relu
+            bare = i < last and counter and self.norms is None and self.activation is F.relu and _stands_alone(layer, ROF_GCNConv)
             h = layer.convolve(h, inputInfo) if bare else layer(h, inputInfo)
             if i == last:
                 break
@@ -191,10 +204,12 @@ class ROF_GIN(torch.nn.Module):
             if i + 1 == len(self.mlps):
                 break
             drop = dict(p=self.dropout, seed=seed, step=step + (i << 40), row_offset=row_offset, training=self.training)
+            done = False
             if self.norms is not None:
-                m = self.norms[i]
-                h = N.layer_norm(h, m.weight, m.bias, m.eps, relu=True, **drop)
-            elif self.dropout > 0:
+                h, done = _norm_relu_dropout(self.norms[i], h, True, drop)
+            if done:
+                continue
+            if self.dropout > 0:
                 h = N.dropout(h, relu=True, **drop)
             else:
                 h = F.relu(h)

@@ -6,7 +6,9 @@ import torch.nn.functional as F
 
 import norm_reference as R
 from artifact_b200 import _native, graphs, norm, search
-from artifact_b200.models import ROF_GCN, ROF_inputInfo
+from artifact_b200.models import ROF_GCN, ROF_GIN, ROF_inputInfo
+from artifact_b200.plan import AggregationPlan
+from conftest import load_golden
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -170,3 +172,71 @@ def test_the_plain_stack_keeps_its_pass_without_gradients():
     with torch.no_grad():
         got = model(x, info)
         assert torch.equal(got, model.eval()(x, info))
+
+
+def test_hooks_of_a_stack_see_their_modules():
+    """with a hook on it a norm or a layer is called as it stands, and the stack's result stays"""
+    for norm_kind in ("layer", None):
+        model, info, x = gcn(norm_kind)
+        for m in model.norms or ():
+            m.bias.data.uniform_(-0.5, 0.5)
+        for m in model.layers:
+            m.bias.data.uniform_(-0.1, 0.1)
+        kw = dict(seed=11, step=4)
+        want = model(x, info, **kw)
+        seen = {}
+        handles = [m.register_forward_hook(lambda mod, args, out, k=k: seen.__setitem__(k, (args[0].detach(), out.detach())))
+                   for k, m in [(f"layer{i}", m) for i, m in enumerate(model.layers)] + [(f"norm{i}", m) for i, m in enumerate(model.norms or ())]]
+        got = model(x, info, **kw)
+        assert len(seen) == 3 + (2 if norm_kind else 0)
+        for i, layer in enumerate(model.layers):
+            given, out = seen[f"layer{i}"]
+            assert torch.equal(out, layer(given, info))                # with its bias, without what follows
+        for i, m in enumerate(model.norms or ()):
+            given, out = seen[f"norm{i}"]
+            assert torch.equal(given, seen[f"layer{i}"][1]) and torch.equal(out, norm.layer_norm(given, m.weight, m.bias))
+        assert (got - want).abs().max() <= 2e-5 * want.abs().max()
+        for h in handles:
+            h.remove()
+        assert torch.equal(model(x, info, **kw), want)
+
+
+@pytest.mark.parametrize("make", [lambda: torch.nn.LayerNorm(16), lambda: torch.nn.Identity(), lambda: torch.nn.BatchNorm1d(16),
+                                  lambda: norm.LayerNorm(16, relu=True)])
+def test_replaced_norms_of_a_stack_are_called(make):
+    model, info, x = gcn()
+    for i in range(2):
+        model.norms[i] = make().to(DEV)
+    got = model(x, info, seed=11, step=4)
+    h = x
+    for i, layer in enumerate(model.layers):
+        h = layer(h, info)
+        if i < 2:
+            mask = torch.from_numpy(R.keep_mask(x.size(0), 16, 0.4, 11, 4 + (i << 40))).to(DEV)
+            h = F.relu(model.norms[i](h)) * mask / 0.6
+    assert (got - h).abs().max() <= 2e-5 * h.abs().max()
+
+
+def test_hooked_and_replaced_norms_of_a_gin_stack():
+    g = load_golden("c3_n1500_ps3")
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(DEV)  # noqa: E731
+    plan = AggregationPlan.from_parts(g["N"], t(g["indices_src"]), t(g["indptr_dst"]), t(np.arange(g["N"])))
+    torch.manual_seed(0)
+    model = ROF_GIN(20, 32, 5, norm="layer", dropout=0.25).to(DEV)
+    x, kw = randn(g["N"], 20, seed=1), dict(seed=6, step=1)
+    want, seen = model(x, plan, **kw), []
+    handle = model.norms[0].register_forward_hook(lambda mod, args, out: seen.append(torch.equal(out, norm.layer_norm(args[0], mod.weight, mod.bias))))
+    assert (model(x, plan, **kw) - want).abs().max() <= 2e-5 * want.abs().max() and seen == [True]
+    handle.remove()
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: seen.append(mod))
+    try:
+        model(x, plan, **kw)
+    finally:
+        handle.remove()
+    assert all(m in seen for m in model.norms)
+    model.norms[1] = torch.nn.LayerNorm(32).to(DEV)
+    assert (model(x, plan, **kw) - want).abs().max() <= 2e-5 * want.abs().max()
+    model.norms[0] = norm.LayerNorm(32, p=1.0).to(DEV)                  # its own dropout zeroes everything
+    model.norms[0].register_forward_hook(lambda mod, args, out: seen.append(bool((out == 0).all())))
+    model(x, plan, **kw)
+    assert seen[-1] is True
