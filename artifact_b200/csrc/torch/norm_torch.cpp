@@ -3,6 +3,7 @@
 // one of them is 10 us of kernels, and an autograd node written in Python costs 60 us more than one that is not.
 //
 // artifact_b200/norm.py documents the operators and hands their arguments through.
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -24,6 +25,14 @@ using torch::autograd::variable_list;
 using MaybeTensor = std::optional<Tensor>;
 
 int dtype_code(at::ScalarType t) { return t == at::kFloat ? ROF_DTYPE_F32 : t == at::kBFloat16 ? ROF_DTYPE_BF16 : ROF_DTYPE_F16; }
+
+// What the operators do not offer is refused: without a node of its own the result would carry no tangent, and a trace records the
+// allocation of the result alone.
+void check_call(const char* who, const Tensor& x, const MaybeTensor& a, const MaybeTensor& b) {
+  const auto dual = [](const Tensor& t) { return t._fw_grad(0).defined(); };
+  TORCH_CHECK(!dual(x) && !(a.has_value() && dual(*a)) && !(b.has_value() && dual(*b)), who, " has no forward-mode derivative");
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), who, " cannot be traced (torch.jit.trace)");
+}
 
 void check_matrix(const Tensor& x) {
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
@@ -186,6 +195,7 @@ bool needs_graph(const Tensor& x, const MaybeTensor& a, const MaybeTensor& b) {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, bool relu, double p, uint64_t seed,
                   uint64_t step, int64_t first_row, const MaybeTensor& step_tensor) {
+  check_call("layer_norm", x, weight, bias);
   check_matrix(x);
   check_vector(weight, "weight", x);
   check_vector(bias, "bias", x);
@@ -258,6 +268,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, const MaybeTensor& bias, bool relu, double p, uint64_t seed, uint64_t step, int64_t first_row,
                const MaybeTensor& step_tensor) {
+  check_call("dropout", x, bias, std::nullopt);
   check_matrix(x);
   check_vector(bias, "bias", x);
   const Drop drop{p, (int64_t)seed, (int64_t)step, first_row};

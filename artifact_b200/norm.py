@@ -49,7 +49,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, p=0.0, seed=None
     x: a CUDA tensor [..., width] of float32, bfloat16 or float16 with any strides; weight, bias: vectors of `width`
     entries, float32 or of x's type, or None; eps >= 0.  relu: apply the ReLU.  p, seed, step, row_offset: the
     dropout behind it (see `dropout`), only where `training`.  Returns a contiguous tensor like x; gradients flow to x, weight
-    and bias (once: a second derivative is not offered)."""
+    and bias (once: a second derivative is not offered, nor are forward-mode derivatives and torch.jit.trace; all are refused)."""
     return _native.torch_ops().layer_norm(x, weight, bias, eps, bool(relu), *_drop_args(p, seed, step, row_offset, training))
 
 

@@ -127,6 +127,22 @@ def test_rows_whose_variance_passes_the_range_of_32_bits(dtype, dim):
     assert torch.equal(norm.layer_norm(x, w, b, eps=float("inf")), b.to(dtype).expand(7, dim))
 
 
+def test_forward_mode_and_traces_are_refused():
+    x, v = randn(4, 8, seed=1), randn(8, seed=2)
+    for call in (lambda a, b: norm.layer_norm(a, b), lambda a, b: norm.layer_norm(a, None, b, relu=True), lambda a, b: norm.dropout(a, bias=b)):
+        with torch.autograd.forward_ad.dual_level():
+            for a, b in ((torch.autograd.forward_ad.make_dual(x, x), v), (x, torch.autograd.forward_ad.make_dual(v, v))):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(a, b)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(a, b)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (x, v))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x, v), (x, v))
+        assert torch.isfinite(call(x, v)).all()
+
+
 # ---- in the models --------------------------------------------------------------------------------
 def gcn(norm_kind="layer", source="counter", dropout=0.4, activation=F.relu, layers=2):
     g = graphs.config1()

@@ -1,0 +1,30 @@
+"""Layer norm and dropout without a GPU at calls that the other tests do not make."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from artifact_b200 import norm
+
+
+@pytest.mark.parametrize("call, takes_v", [(lambda x, v: norm.layer_norm(x), False), (lambda x, v: norm.layer_norm(x, v), True),
+                                           (lambda x, v: norm.layer_norm(x, None, v), True), (lambda x, v: norm.dropout(x), False),
+                                           (lambda x, v: norm.dropout(x, 0.5, seed=1, bias=v), True)])
+@pytest.mark.parametrize("grads", [False, True])
+def test_forward_mode_is_refused(call, takes_v, grads):
+    """not answered without a tangent"""
+    x, v = torch.ones(4, 8, requires_grad=grads), torch.ones(8)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            call(fwAD.make_dual(x, torch.ones(4, 8)), v)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative" if takes_v else "CUDA tensor"):
+            call(x, fwAD.make_dual(v, torch.ones(8)))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        call(x, v)
+
+
+@pytest.mark.parametrize("call", [lambda x: norm.layer_norm(x, relu=True), lambda x: norm.dropout(x, 0.5, seed=1),
+                                  lambda x: norm.LayerNorm(8)(x), lambda x: norm.Dropout(0.0)(x)])
+def test_traces_are_refused(call):
+    """a trace would hold the allocation of the result and nothing that fills it"""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, torch.ones(4, 8))
