@@ -52,6 +52,10 @@ inline int column_blocks_cap(int64_t rows, int dim) {
   return (int)std::min<int64_t>(cap, (std::max<int64_t>(rows, 1) + 7) / 8 * 8);
 }
 
+// Whether a 16-byte vector of `vec` elements whose first is in column c of a row ends in the matrix, with `behind` rows after its own.  A vector
+// that passes the end of its row reaches up to vec - 1 elements further: into rows of one column and more that many rows follow.
+__host__ __device__ inline bool ends_in_matrix(int64_t behind, int c, int dim, int vec) { return c + vec <= dim || behind >= vec; }
+
 // The tile kernels (norm_tile.cuh).
 enum TileMode { kNormForward, kNormForwardHidden, kNormBackward, kNormBackwardHidden, kDropForward, kDropBackward };
 

@@ -43,11 +43,11 @@ union Pack {
   __device__ Pack() {}
 };
 
-// Columns [c, c + VEC) of a row, c + VEC > 0.  Partial vectors hold what the 16 bytes hold, the neighbouring row's elements or what
-// precedes the matrix in its allocation; behind the end of the matrix (`last`: its last row) nothing is read.
+// Columns [c, c + VEC) of a row, c + VEC > 0, with `behind` rows after it.  Partial vectors hold what the 16 bytes hold, the neighbouring
+// row's elements or what precedes the matrix in its allocation; behind the end of the matrix nothing is read.
 template <class T, bool EDGE>
-__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim, bool last) {
-  if (!EDGE || !last || c + kVec<T> <= dim) {
+__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim, int64_t behind) {
+  if (!EDGE || ends_in_matrix(behind, c, dim, kVec<T>)) {
     out.raw = *reinterpret_cast<const uint4*>(row + c);
   } else {
 #pragma unroll

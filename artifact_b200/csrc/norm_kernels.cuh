@@ -583,9 +583,9 @@ __global__ void __launch_bounds__(256, drop_row_blocks<T, BACK && !DRAW, EDGE>()
       for (int u = 0; u < U; ++u) {
         in[u].raw = yy[u].raw = make_uint4(0, 0, 0, 0);
         if (r + u * stride < a.rows) {
-          const bool last = r + u * stride == a.rows - 1;
-          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim, last);
-          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim, last);
+          const int64_t behind = a.rows - 1 - (r + u * stride);
+          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim, behind);
+          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim, behind);
         }
       }
       float2 o[U][V / 2];

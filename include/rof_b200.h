@@ -302,7 +302,8 @@ int rof_shared_free(void* ptr);
  * The operators between two graph layers (no counterpart in upstream, whose model calls torch for its dropout,
  * ROF_main.py:192-200): layer norm, dropout, and the two in one pass with the ReLU between them.  Matrices are
  * row-major with `dim` columns (at most 2^30) and a row stride in elements, of one of the types below (at least aligned to
- * their elements; rows whose address and stride are multiples of 16 bytes run on 128-bit loads); vectors
+ * their elements; rows whose address and stride are multiples of 16 bytes run on 128-bit loads; of the aligned 16 bytes in which a
+ * matrix begins all may be read, behind its end nothing is); vectors
  * (weight, bias and their gradients) are [dim], 32-bit or of the matrix's type (`vdtype`).  Sums, statistics and all arithmetic are
  * 32-bit; a result is rounded to the matrix's type once.  The calls only enqueue work on `stream`, on the
  * current device, allocate nothing, and give the same result bit for bit every time.

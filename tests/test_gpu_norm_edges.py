@@ -60,6 +60,30 @@ def test_dropout_gradients_in_place_with_a_bias_gradient(dtype, relu, rows, dim)
             R.assert_within(got, want[name], f"ld {ld} {name}")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [1, 2, 3, 5, 7, 9])
+def test_dropout_of_rows_shorter_than_a_vector(dtype, dim):
+    """off the 16-byte boundaries: rows before the last reach the matrix's end too, and what lies around the outputs stays"""
+    b = randn(dim, seed=3)
+    for rows in (1, 2, 5, 19):
+        for lead in (0, 1, 2, 3):
+            for ld in (dim, dim + 1):
+                laid = lambda: torch.full((8 + lead + rows * ld + 8,), 7.0, dtype=dtype, device=DEV)  # noqa: E731
+                view = lambda buf: buf.as_strided((rows, dim), (ld, 1), 8 + lead)  # noqa: E731
+                x, dy = view(laid()), view(laid())
+                x.copy_(randn(rows, dim, seed=1, dtype=dtype))
+                dy.copy_(randn(rows, dim, seed=2, dtype=dtype))
+                ybuf, gbuf = laid(), laid()
+                for relu in (0, 1):
+                    want = R.dropout_reference(x, b, bool(relu), 0.4, 9, 3, dy=dy)
+                    db = c_dropout(x, b, dy, view(ybuf), view(gbuf), relu, _native.Dropout(0.4, 9, 3, None, 0))
+                    for got, name in ((view(ybuf), "y"), (view(gbuf), "dx"), (db, "db")):
+                        R.assert_within(got, want[name], f"{rows} {lead} {ld} {name}")
+                for buf in (ybuf, gbuf):
+                    view(buf).fill_(7.0)
+                    assert (buf == 7.0).all()
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("p", [0.0, 0.5])
 @pytest.mark.parametrize("dim", [8, 47, 64, 100, 301, 602, 2049, 4097])

@@ -1,9 +1,13 @@
 """Layer norm and dropout without a GPU at calls that the other tests do not make."""
+import os
+import subprocess
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from artifact_b200 import norm
+from artifact_b200 import build, norm
+from conftest import ROOT
 
 
 @pytest.mark.parametrize("call, takes_v", [(lambda x, v: norm.layer_norm(x), False), (lambda x, v: norm.layer_norm(x, v), True),
@@ -28,3 +32,13 @@ def test_traces_are_refused(call):
     """a trace would hold the allocation of the result and nothing that fills it"""
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(call, torch.ones(4, 8))
+
+
+def test_no_vector_is_read_behind_the_matrix(tmp_path):
+    """rows shorter than a vector: more rows than the last reach behind the matrix's end"""
+    exe = str(tmp_path / "matrix_ends")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(build._nvcc())))
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", build.CSRC, "-isystem", os.path.join(cuda, "include"),
+                           os.path.join(ROOT, "tests", "abi", "matrix_ends.cpp"), "-o", exe])
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and " wrong 0 held 0" in out.stdout, out.stdout
