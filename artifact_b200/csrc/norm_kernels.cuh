@@ -355,13 +355,14 @@ __global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 
 // out[i] = sum over the blocks' partial[block][i] for i in [0, width): eight runs of blocks per column, added in order.  Columns
 // up to `split` go to `first`, the others to `second`.
 template <class T>
-__global__ void __launch_bounds__(256) join_columns_kernel(const float* partial, int blocks, int width, int split, void* first, void* second, int f32) {
+__global__ void __launch_bounds__(256) join_columns_kernel(const float* partial, int blocks, int64_t width, int64_t split, void* first, void* second, int f32) {
   __shared__ float part[8][33];
-  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, i = blockIdx.x * 32 + x;
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + x;
   float sum = 0.0f;
   if (i < width) {
 #pragma unroll 8
-    for (int k = run; k < blocks; k += 8) sum += partial[(int64_t)k * width + i];
+    for (int k = run; k < blocks; k += 8) sum += partial[k * width + i];
   }
   part[run][x] = sum;
   __syncthreads();
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(256) join_columns_kernel(const float* partial,
 #pragma unroll
     for (int k = 1; k < 8; ++k) sum += part[k][x];
     void* out = i < split ? first : second;
-    if (out != nullptr) vector_put<T>(out, f32, i < split ? i : i - split, sum);
+    if (out != nullptr) vector_put<T>(out, f32, (int)(i < split ? i : i - split), sum);
   }
 }
 
@@ -845,8 +846,8 @@ inline TileLauncher tile_launcher(__nv_bfloat16) { return tile_launcher_bf16; }
 inline TileLauncher tile_launcher(__half) { return tile_launcher_f16; }
 
 template <class T>
-cudaError_t launch_join(const float* partial, int blocks, int width, int split, void* first, void* second, int f32, cudaStream_t stream) {
-  join_columns_kernel<T><<<(width + 31) / 32, 256, 0, stream>>>(partial, blocks, width, split, first, second, f32);
+cudaError_t launch_join(const float* partial, int blocks, int64_t width, int64_t split, void* first, void* second, int f32, cudaStream_t stream) {
+  join_columns_kernel<T><<<(unsigned)((width + 31) / 32), 256, 0, stream>>>(partial, blocks, width, split, first, second, f32);
   return cudaGetLastError();
 }
 
@@ -898,7 +899,7 @@ cudaError_t launch_norm_backward(const NormArgs& given, cudaStream_t stream) {
     }
   }
   if (a.partial == nullptr) return cudaGetLastError();
-  return launch_join<T>(a.partial, blocks, 2 * a.dim, a.dim, a.dweight, a.dbias, a.wf32, stream);
+  return launch_join<T>(a.partial, blocks, 2 * (int64_t)a.dim, a.dim, a.dweight, a.dbias, a.wf32, stream);
 }
 
 // As many blocks as run at once; a multiple of 8, so that a thread's rows keep their distance to the 16-byte boundaries.

@@ -151,6 +151,33 @@ def test_rows_whose_variance_passes_the_range_of_32_bits(dtype, dim):
     assert torch.equal(norm.layer_norm(x, w, b, eps=float("inf")), b.to(dtype).expand(7, dim))
 
 
+def test_column_sums_of_the_widest_rows():
+    """2^30 columns: the two vectors' gradients together have 2^31 entries"""
+    lib, s, dim = _native.cuda(), torch.cuda.current_stream().cuda_stream, 2 ** 30
+    n = lib.rof_layer_norm_workspace_bytes(1, dim)
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < n + 20 * 2 ** 30:
+        pytest.skip("needs 84 GB")
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.empty((1, dim), dtype=BF16, device=DEV).normal_(generator=gen) for _ in range(2))
+    dw, db = (torch.full((dim,), float("nan"), dtype=BF16, device=DEV) for _ in range(2))
+    ws, stats = torch.empty((n,), dtype=torch.uint8, device=DEV), torch.tensor([0.25, 0.5], device=DEV)
+    for d in (dim, dim - 8):
+        dw.fill_(float("nan"))
+        db.fill_(float("nan"))
+        _native.check(lib.rof_layer_norm_backward(1, dy.data_ptr(), d, x.data_ptr(), d, 1, d, 1, None, None, stats.data_ptr(), 0, None,
+                                                  None, d, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, s))
+        assert torch.equal(db[:d], dy[0, :d]) and torch.isnan(db[d:]).all() and torch.isnan(dw[d:]).all()
+        for i in range(0, d, 2 ** 26):
+            e = min(i + 2 ** 26, d)
+            assert torch.equal(dw[i:e], ((x[0, i:e].float() - 0.25) * 0.5 * dy[0, i:e].float()).to(BF16))
+        db.fill_(float("nan"))
+        _native.check(lib.rof_dropout_backward(1, dy.data_ptr(), d, None, d, 1, d, 1, 0, None, None, d, db.data_ptr(), ws.data_ptr(), n, s))
+        assert torch.equal(db[:d], dy[0, :d])
+    del ws
+    torch.cuda.empty_cache()
+
+
 def test_forward_mode_and_traces_are_refused():
     x, v = randn(4, 8, seed=1), randn(8, seed=2)
     for call in (lambda a, b: norm.layer_norm(a, b), lambda a, b: norm.layer_norm(a, None, b, relu=True), lambda a, b: norm.dropout(a, bias=b)):
