@@ -9,6 +9,7 @@ from artifact_b200 import _native, graphs, norm, search
 from artifact_b200.models import ROF_GCN, ROF_GIN, ROF_inputInfo
 from artifact_b200.plan import AggregationPlan
 from conftest import load_golden
+from test_gpu_norm import _c_norm, calm_gradient
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -192,6 +193,39 @@ def test_forward_mode_and_traces_are_refused():
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (x, v), (x, v))
         assert torch.isfinite(call(x, v)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [8, 47, 64, 130, 301, 602, 1001])
+def test_calm_gradients_with_strides_through_the_c_abi(dtype, dim):
+    """mixes of how the four matrices lie, with no gradient next to the ReLU's border"""
+    rows, w, b = 41, randn(dim, seed=13, scale=0.3, shift=1.0), randn(dim, seed=14, scale=0.3)
+    x0 = randn(rows, dim, seed=11, dtype=dtype)
+    dy0 = calm_gradient(randn(rows, dim, seed=12, dtype=dtype), x0, w, b, 1e-5)
+    up = -(-dim // 8) * 8
+    want = R.norm_reference(x0, w, b, relu=True, p=0.3, seed=9, step=3, row_offset=4, dy=dy0)
+    layouts = (up, dim, dim + 1, up + 8)
+    for i, lx in enumerate(layouts):
+        for ly in (layouts[i], layouts[(i + 1) % 4], layouts[(i + 2) % 4]):
+            y, dx = padded(torch.zeros_like(x0), ly), padded(torch.zeros_like(x0), lx)
+            dw, db = _c_norm(padded(x0, lx), w, b, padded(dy0, ly), y, dx, 1, _native.Dropout(0.3, 9, 3, None, 4))
+            for got, n in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
+                R.assert_within(got, want[n], f"{lx} {ly} {n}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, dim", [(1, 7), (129, 47), (65, 100), (300, 128), (40, 602), (5, 1031), (1, 70001), (4000, 33)])
+def test_masks_element_by_element(dtype, rows, dim):
+    """zero exactly where the definition is, in 16 bits too, forward and back (values whose size the type can hold)"""
+    x, dy, b = randn(rows, dim, seed=21, dtype=dtype), randn(rows, dim, seed=22, dtype=dtype), randn(dim, seed=23)
+    for bias, relu in ((None, False), (b, False), (None, True), (b, True)):
+        want = R.dropout_reference(x, bias, relu, 0.4, 7, 5, 2, dy=dy)
+        leaf = x.clone().requires_grad_(True)
+        y = norm.dropout(leaf, 0.4, seed=7, step=5, row_offset=2, bias=bias, relu=relu)
+        for got, name in ((y, "y"), (torch.autograd.grad(y, leaf, dy)[0], "dx")):
+            size = np.abs(want[name][0])
+            held = (size == 0) | (size > 4 * R.tiny(dtype))
+            assert held.mean() > 0.99 and ((got == 0).cpu().numpy() == (size == 0))[held].all(), (name, relu)
 
 
 # ---- in the models --------------------------------------------------------------------------------
