@@ -11,6 +11,7 @@ The first two are plain shared objects loaded with ctypes and know nothing of to
 Python module that links against the first and against torch.
 Run ``python -m artifact_b200.build`` (or ``__graft_entry__.build()``).
 """
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -97,6 +98,13 @@ def build_host(force=False, verbose=True):
     return target
 
 
+def torch_root():
+    """the installed torch's folder, where it has its C++ headers; else None (nothing is imported)"""
+    spec = importlib.util.find_spec("torch")
+    root = os.path.dirname(spec.origin) if spec is not None and spec.origin else None
+    return root if root and os.path.exists(os.path.join(root, "include", "torch", "csrc", "autograd", "custom_function.h")) else None
+
+
 def build_torch(force=False, verbose=True):
     cuda = build_cuda(verbose=verbose)
     src = os.path.join(CSRC, "torch", "norm_torch.cpp")
@@ -118,9 +126,13 @@ def build_torch(force=False, verbose=True):
 
 
 def build_all(force=False, verbose=True):
-    """-> the CUDA library and the host library (rof_torch.so is built beside them)"""
+    """-> the CUDA library and the host library (rof_torch.so is built beside them, where torch and its headers are installed)"""
     libs = build_cuda(force, verbose), build_host(force, verbose)
-    build_torch(force, verbose)
+    if torch_root() is not None:
+        build_torch(force, verbose)
+    else:
+        print("rof_torch.so is not built: torch with its C++ headers is not installed (artifact_b200.norm needs it; the C ABI does not)",
+              file=sys.stderr, flush=True)
     return libs
 
 

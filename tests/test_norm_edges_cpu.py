@@ -42,3 +42,15 @@ def test_no_vector_is_read_behind_the_matrix(tmp_path):
                            os.path.join(ROOT, "tests", "abi", "matrix_ends.cpp"), "-o", exe])
     out = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and " wrong 0 held 0" in out.stdout, out.stdout
+
+
+def test_the_c_abi_builds_without_torch(monkeypatch, capsys):
+    """without torch's headers the two libraries that know nothing of torch are built as before"""
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose: None)
+    monkeypatch.setattr(build, "_stale", lambda target, deps: True)
+    found = build.importlib.util.find_spec
+    assert build.torch_root() == os.path.dirname(torch.__file__)
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name, *more: None if name == "torch" else found(name, *more))
+    monkeypatch.setitem(__import__("sys").modules, "torch", None)         # `import torch` raises
+    assert build.build_all(verbose=False) == (build.cuda_lib_path(), build.host_lib_path())
+    assert "rof_torch.so is not built" in capsys.readouterr().err
