@@ -105,11 +105,22 @@ def torch_root():
     return root if root and os.path.exists(os.path.join(root, "include", "torch", "csrc", "autograd", "custom_function.h")) else None
 
 
+def _torch_stamp():
+    """which torch rof_torch.so is built against: its folder and version"""
+    root = torch_root()
+    if root is None:
+        raise RuntimeError("rof_torch.so needs an installed torch with its C++ headers")
+    with open(os.path.join(root, "version.py")) as f:
+        return root + "\n" + f.read()
+
+
 def build_torch(force=False, verbose=True):
     cuda = build_cuda(verbose=verbose)
     src = os.path.join(CSRC, "torch", "norm_torch.cpp")
-    target = torch_lib_path()
-    if not force and not _stale(target, [src, os.path.join(INCLUDE, "rof_b200.h"), os.path.abspath(__file__)]):
+    target, stamp = torch_lib_path(), os.path.join(LIB, "rof_torch.stamp")
+    against = _torch_stamp()
+    same = os.path.exists(stamp) and open(stamp).read() == against
+    if not force and same and not _stale(target, [src, os.path.join(INCLUDE, "rof_b200.h"), os.path.abspath(__file__)]):
         return target
     import torch
     root = os.path.dirname(os.path.abspath(torch.__file__))
@@ -122,6 +133,8 @@ def build_torch(force=False, verbose=True):
     cmd += [src, "-o", target, "-L" + LIB, "-l:" + os.path.basename(cuda), "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(root, "lib"),
             "-Wl,-rpath," + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
     _run(cmd, verbose)
+    with open(stamp, "w") as f:
+        f.write(against)
     return target
 
 

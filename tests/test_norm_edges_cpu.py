@@ -54,3 +54,17 @@ def test_the_c_abi_builds_without_torch(monkeypatch, capsys):
     monkeypatch.setitem(__import__("sys").modules, "torch", None)         # `import torch` raises
     assert build.build_all(verbose=False) == (build.cuda_lib_path(), build.host_lib_path())
     assert "rof_torch.so is not built" in capsys.readouterr().err
+
+
+def test_the_torch_binding_is_built_anew_for_another_torch(monkeypatch, tmp_path):
+    runs = []
+    monkeypatch.setattr(build, "LIB", str(tmp_path))
+    monkeypatch.setattr(build, "build_cuda", lambda **kw: "librof_b200.so")
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose: (runs.append(cmd), open(build.torch_lib_path(), "w").close()))
+    build.build_torch(verbose=False)
+    build.build_torch(verbose=False)
+    assert len(runs) == 1
+    monkeypatch.setattr(build, "_torch_stamp", lambda: "another")
+    build.build_torch(verbose=False)
+    build.build_torch(verbose=False)
+    assert len(runs) == 2
