@@ -24,7 +24,7 @@ def draw_seed():
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured dropout needs a seed: one drawn now would be the same on every replay "
                            "(give `seed`, and a `step` tensor that the graph adds to)")
-    return int(torch.empty((), dtype=torch.int64).random_())
+    return int(torch.empty((), dtype=torch.int64, device="cpu").random_())
 
 
 def _drop_args(p, seed, step, row_offset, training):

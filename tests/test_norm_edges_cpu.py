@@ -68,3 +68,11 @@ def test_the_torch_binding_is_built_anew_for_another_torch(monkeypatch, tmp_path
     build.build_torch(verbose=False)
     build.build_torch(verbose=False)
     assert len(runs) == 2
+
+
+def test_seeds_come_from_the_cpu_whatever_the_default_device():
+    torch.manual_seed(5)
+    want = [norm.draw_seed() for _ in range(2)]
+    torch.manual_seed(5)
+    with torch.device("meta"):                                           # (a GPU in a user's program)
+        assert [norm.draw_seed() for _ in range(2)] == want
