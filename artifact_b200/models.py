@@ -110,6 +110,10 @@ class ROF_GCN(torch.nn.Module):
         # (not among the children without a norm: the state of such a stack keeps its names)
         self.norms = torch.nn.ModuleList(N.LayerNorm(d) for d in dims[1:-1]) if norm is not None else None
 
+    def __setstate__(self, state):
+        # (a stack that was saved whole before it could have these)
+        super().__setstate__({"norms": None, "dropout_source": "torch", **state} if "norms" not in state["_modules"] else state)
+
     def _between(self, h, i, bias, drop):
         """what stands between layer i and the next: norm, activation, dropout (`drop`: its keywords, or None)"""
         relu = self.activation is F.relu
@@ -194,6 +198,9 @@ class ROF_GIN(torch.nn.Module):
             for a, b in zip(dims[:-1], dims[1:]))
         self.eps, self.dropout = eps, dropout
         self.norms = torch.nn.ModuleList(N.LayerNorm(d) for d in dims[1:-1]) if norm is not None else None
+
+    def __setstate__(self, state):
+        super().__setstate__({"norms": None, "dropout": 0.0, **state} if "norms" not in state["_modules"] else state)
 
     def forward(self, features, plan: AggregationPlan, plan_t=None, seed=None, step=0, row_offset=0):
         h = features

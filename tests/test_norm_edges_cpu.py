@@ -1,5 +1,7 @@
 """Layer norm and dropout without a GPU at calls that the other tests do not make."""
+import io
 import os
+import pickle
 import subprocess
 
 import pytest
@@ -7,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 from artifact_b200 import build, norm
+from artifact_b200.models import ROF_GCN, ROF_GIN
 from conftest import ROOT
 
 
@@ -76,3 +79,18 @@ def test_seeds_come_from_the_cpu_whatever_the_default_device():
     torch.manual_seed(5)
     with torch.device("meta"):                                           # (a GPU in a user's program)
         assert [norm.draw_seed() for _ in range(2)] == want
+
+
+def test_models_saved_before_they_had_norms_load():
+    """whole stacks pickled without the attributes that norm and dropout_source brought"""
+    for model, made in ((ROF_GCN(8, 4, 2, 1), ("norms", "dropout_source")), (ROF_GIN(8, 4, 2), ("norms", "dropout"))):
+        for k in made:
+            delattr(model, k)
+        buf = io.BytesIO()
+        torch.save(model, buf)
+        buf.seek(0)
+        got = torch.load(buf, weights_only=False)
+        assert got.norms is None and (got.dropout_source == "torch" if isinstance(got, ROF_GCN) else got.dropout == 0.0)
+    for model in (ROF_GCN(8, 4, 2, 1, norm="layer", dropout_source="counter", dropout=0.3), ROF_GIN(8, 4, 2, norm="layer", dropout=0.3)):
+        got = pickle.loads(pickle.dumps(model))
+        assert got.dropout == 0.3 and len(got.norms) == len(model.norms) and getattr(got, "dropout_source", "counter") == "counter"
