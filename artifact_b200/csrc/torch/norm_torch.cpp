@@ -61,7 +61,7 @@ struct Drop {
 void check_drop(const Drop& d, const MaybeTensor& step, const Tensor& x) {
   TORCH_CHECK_VALUE(d.p >= 0.0 && d.p <= 1.0, "p must be in [0, 1], got ", d.p);
   TORCH_CHECK_VALUE(d.first_row >= 0, "row_offset must not be negative, got ", d.first_row);
-  TORCH_CHECK(!step.has_value() || (step->scalar_type() == at::kLong && step->numel() == 1 && step->device() == x.device()),
+  TORCH_CHECK(!step.has_value() || (step->scalar_type() == at::kLong && step->numel() == 1 && step->device() == x.device() && !step->is_neg()),
               "step must be a number or a one-element int64 tensor on x's device");
 }
 
@@ -70,7 +70,8 @@ void check_status(int status) {
 }
 
 // x as [rows, width] with unit column stride: a view where its layout allows it, else a copy
-Tensor rows_of(const Tensor& x) {
+Tensor rows_of(const Tensor& given) {
+  const Tensor x = given.resolve_neg();               // (what such a view holds is not what its memory holds)
   const Tensor v = x.dim() == 2 ? x : x.dim() == 1 ? x.unsqueeze(0) : x.flatten(0, -2);
   if (v.is_contiguous() || ((v.stride(1) == 1 || v.size(1) <= 1) && (v.stride(0) >= v.size(1) || v.size(0) <= 1))) return v;
   return v.contiguous();
@@ -101,7 +102,7 @@ at::ScalarType kind_of(const Tensor& weight, const Tensor& bias) {
   return weight.scalar_type() == bias.scalar_type() ? weight.scalar_type() : at::kFloat;
 }
 
-Tensor vector_of(const Tensor& v, at::ScalarType kind) { return v.defined() ? v.to(kind).contiguous() : v; }
+Tensor vector_of(const Tensor& v, at::ScalarType kind) { return v.defined() ? v.to(kind).resolve_neg().contiguous() : v; }
 
 const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mutable_pointer(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -212,7 +213,7 @@ Tensor dropout_forward(const Tensor& x, const Tensor& bias, bool relu, const Dro
   const c10::DeviceGuard guard(x.device());
   const Tensor v = rows_of(x), y = empty_like_rows(x);
   const int width = width_of(v);
-  const Tensor b = bias.defined() ? bias.contiguous() : bias;
+  const Tensor b = bias.defined() ? vector_of(bias, bias.scalar_type()) : bias;
   const rof_dropout d = drop.c(step);
   check_status(rof_dropout_forward(dtype_code(x.scalar_type()), v.const_data_ptr(), v.stride(0), v.size(0), width,
                                    dtype_code(b.defined() ? b.scalar_type() : at::kFloat), pointer(b), relu, drop.p > 0.0 ? &d : nullptr,

@@ -228,6 +228,19 @@ def test_masks_element_by_element(dtype, rows, dim):
             assert held.mean() > 0.99 and ((got == 0).cpu().numpy() == (size == 0))[held].all(), (name, relu)
 
 
+def test_lazily_negated_tensors():
+    x, w, b, dy = randn(33, 24, seed=1), randn(24, seed=2), randn(24, seed=3), randn(33, 24, seed=4)
+    n = [torch._neg_view(-t) for t in (x, w, b, dy)]
+
+    def both(x, w, b, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y, d = norm.layer_norm(*leaves), norm.dropout(leaves[0], 0.3, seed=1, bias=leaves[2], relu=True)
+        return y, d, *torch.autograd.grad(y, leaves, dy), *torch.autograd.grad(d, (leaves[0], leaves[2]), dy)
+
+    for got, want in zip(both(*n), both(x, w, b, dy)):
+        assert torch.equal(got, want)
+
+
 # ---- in the models --------------------------------------------------------------------------------
 def gcn(norm_kind="layer", source="counter", dropout=0.4, activation=F.relu, layers=2):
     g = graphs.config1()

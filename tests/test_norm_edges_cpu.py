@@ -8,7 +8,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from artifact_b200 import build, norm
+from artifact_b200 import _native, build, norm
 from artifact_b200.models import ROF_GCN, ROF_GIN
 from conftest import ROOT
 
@@ -94,3 +94,12 @@ def test_models_saved_before_they_had_norms_load():
     for model in (ROF_GCN(8, 4, 2, 1, norm="layer", dropout_source="counter", dropout=0.3), ROF_GIN(8, 4, 2, norm="layer", dropout=0.3)):
         got = pickle.loads(pickle.dumps(model))
         assert got.dropout == 0.3 and len(got.norms) == len(model.norms) and getattr(got, "dropout_source", "counter") == "counter"
+
+
+def test_lazily_negated_rows_are_read_negated():
+    """a view whose memory holds the negatives (the imaginary part of a conjugate)"""
+    rows_of = _native.torch_ops().rows_of
+    x = torch.arange(12.0).view(3, 4)
+    for v in (torch._neg_view(x), torch._neg_view(x)[:, :3], torch._neg_view(x)[0], torch.randn(4, 1, dtype=torch.complex64).conj().imag):
+        r = rows_of(v)
+        assert v.is_neg() and not r.is_neg() and torch.equal(r.view_as(v) if v.dim() == 2 else r[0], v.clone())
