@@ -144,6 +144,14 @@ variable_list once(variable_list grads, const char* who) {
   return (*error)(std::move(inputs));
 }
 
+// What a backward pass gets back of what was saved.  Hooks on saved tensors may hand back something else, which the kernels must not
+// read: they get pointers.
+void check_saved(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef sizes, const Tensor& dy) {
+  TORCH_CHECK(t.defined() && t.device() == dy.device() && t.scalar_type() == type && t.sizes() == sizes, "a hook on saved tensors returned ",
+              t.defined() ? t.sizes() : at::IntArrayRef(), " ", t.defined() ? c10::toString(t.scalar_type()) : "nothing", " for ", name,
+              ", not what was saved");
+}
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, bool relu,
                         double p, int64_t seed, int64_t step, int64_t first_row, const MaybeTensor& step_tensor) {
@@ -156,7 +164,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &v = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+    const Tensor &weight = saved[1], &bias = saved[2];
     const auto numbers = ctx->saved_data["drop"].toIntVector();
     const Drop drop{ctx->saved_data["p"].toDouble(), numbers[0], numbers[1], numbers[2]};
     variable_list out(10);
@@ -166,10 +174,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                need_b = bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1);
     {
       const at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(v.device());
-      const int64_t rows = v.size(0);
-      const int width = (int)v.size(1);
-      const Tensor dy = laid_like(rows_of(grads[0]), v);
+      const c10::DeviceGuard guard(grads[0].device());
+      const Tensor g = rows_of(grads[0]);
+      const int64_t rows = g.size(0);
+      const int width = (int)g.size(1);
+      check_saved(saved[0], "x", g.scalar_type(), {rows, width}, g);
+      check_saved(saved[3], "the rows' statistics", at::kFloat, {rows, 2}, g);
+      check_vector(weight.defined() ? MaybeTensor(weight) : std::nullopt, "weight", g);
+      check_vector(bias.defined() ? MaybeTensor(bias) : std::nullopt, "bias", g);
+      check_drop(drop, saved[4].defined() ? MaybeTensor(saved[4]) : std::nullopt, g);
+      const Tensor v = rows_of(saved[0]), stats = saved[3].contiguous(), dy = laid_like(g, v);
       const at::ScalarType kind = kind_of(weight, bias);
       const Tensor w = vector_of(weight, kind), b = vector_of(bias, kind);
       Tensor dx, dw, db, ws;
@@ -247,6 +261,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
       Tensor dy = rows_of(grads[0]);
       const int64_t rows = dy.size(0);
       const int width = (int)dy.size(1);
+      if (numbers[3]) check_saved(y, "the output", dy.scalar_type(), grads[0].sizes(), dy);
+      check_drop(drop, saved[1].defined() ? MaybeTensor(saved[1]) : std::nullopt, dy);
       const Tensor yy = y.defined() ? rows_of(y) : y;
       const at::ScalarType kind = numbers[5] ? at::kFloat : dy.scalar_type();
       Tensor dx, db, ws;
@@ -257,7 +273,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         ws = workspace_of(rows, width, dy);
       }
       const rof_dropout d = drop.c(saved[1]);
-      check_status(rof_dropout_backward(dtype_code(dy.scalar_type()), dy.const_data_ptr(), dy.stride(0), pointer(yy), width, rows, width,
+      check_status(rof_dropout_backward(dtype_code(dy.scalar_type()), dy.const_data_ptr(), dy.stride(0), pointer(yy), yy.defined() ? yy.stride(0) : width, rows, width,
                                         dtype_code(kind), (int)numbers[3], drop.p > 0.0 ? &d : nullptr, mutable_pointer(dx), width,
                                         mutable_pointer(db), mutable_pointer(ws), ws.defined() ? ws.numel() : 0, stream_of(dy)));
       out[0] = dx;

@@ -241,6 +241,49 @@ def test_lazily_negated_tensors():
         assert torch.equal(got, want)
 
 
+def test_hooks_on_saved_tensors():
+    """what is saved may travel (to the CPU and back, into another layout); what comes back as something else is refused: the kernels would
+    read its memory"""
+    x, w, b, dy = randn(33, 24, seed=1), randn(24, seed=2), randn(24, seed=3), randn(33, 24, seed=4)
+    step, calm = torch.tensor([3], device=DEV), calm_gradient(dy, x, w, b, 1e-5)
+    kinds = {(33, 24): "rows", (33, 2): "statistics", (24,): "vectors", (1,): "step"}
+
+    def run(op, pack=None, unpack=None):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        if op == "norm":
+            f = lambda: norm.layer_norm(*leaves, relu=True, p=0.3, seed=1, step=step)  # noqa: E731
+        else:
+            leaves.pop(1)
+            f = lambda: norm.dropout(leaves[0], 0.3, seed=1, step=step, bias=leaves[1], relu=op == "relu")  # noqa: E731
+        if pack is None:
+            return torch.autograd.grad(f(), leaves, calm)
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = f()
+        return torch.autograd.grad(y, leaves, calm)
+
+    for op, saves in (("norm", {"rows", "statistics", "vectors", "step"}), ("relu", {"rows", "step"}), ("plain", {"step"})):
+        want, seen = run(op), []
+        if op == "norm":
+            ref = R.norm_reference(x, w, b, relu=True, p=0.3, seed=1, step=3, dy=calm)
+        else:
+            ref = R.dropout_reference(x, b, op == "relu", 0.3, 1, 3, dy=calm)
+        for same, pack, unpack in ((True, lambda t: (seen.append(kinds[tuple(t.shape)]), t.cpu())[1], lambda t: t.to(DEV)),
+                                   (True, lambda t: t.t().contiguous(), lambda t: t.t()),             # columns one after the other
+                                   (False, lambda t: padded(t, t.size(-1) + 3) if t.dim() == 2 else t, lambda t: t)):
+            got = run(op, pack, unpack)
+            # (rows that lie differently against the 16-byte boundaries are added in another order)
+            assert not same or all(torch.equal(a, e) for a, e in zip(got, want)), op
+            for g, name in zip(got, ("dx", "dw", "db") if op == "norm" else ("dx", "db")):
+                R.assert_within(g, ref[name], f"{op} {name}")
+        assert set(seen) == saves
+        for kind in saves:
+            for bad in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:0]):
+                with pytest.raises(RuntimeError, match="hook on saved tensors|must be"):
+                    run(op, lambda t: bad(t) if kinds[tuple(t.shape)] == kind else t, lambda t: t)
+        assert all(torch.equal(a, e) for a, e in zip(run(op), want))
+    torch.cuda.synchronize()
+
+
 # ---- in the models --------------------------------------------------------------------------------
 def gcn(norm_kind="layer", source="counter", dropout=0.4, activation=F.relu, layers=2):
     g = graphs.config1()
