@@ -69,9 +69,12 @@ void check_status(int status) {
   TORCH_CHECK(status == ROF_OK, "rof_b200 status ", status, ": ", rof_last_error());
 }
 
+// a lazily negated view's memory holds the negatives of its values (the question first: the call costs a microsecond)
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // x as [rows, width] with unit column stride: a view where its layout allows it, else a copy
 Tensor rows_of(const Tensor& given) {
-  const Tensor x = given.resolve_neg();               // (what such a view holds is not what its memory holds)
+  const Tensor x = resolved(given);
   const Tensor v = x.dim() == 2 ? x : x.dim() == 1 ? x.unsqueeze(0) : x.flatten(0, -2);
   if (v.is_contiguous() || ((v.stride(1) == 1 || v.size(1) <= 1) && (v.stride(0) >= v.size(1) || v.size(0) <= 1))) return v;
   return v.contiguous();
@@ -102,7 +105,7 @@ at::ScalarType kind_of(const Tensor& weight, const Tensor& bias) {
   return weight.scalar_type() == bias.scalar_type() ? weight.scalar_type() : at::kFloat;
 }
 
-Tensor vector_of(const Tensor& v, at::ScalarType kind) { return v.defined() ? v.to(kind).resolve_neg().contiguous() : v; }
+Tensor vector_of(const Tensor& v, at::ScalarType kind) { return v.defined() ? resolved(v.scalar_type() == kind ? v : v.to(kind)).contiguous() : v; }
 
 const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mutable_pointer(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
