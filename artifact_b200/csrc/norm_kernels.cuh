@@ -473,6 +473,7 @@ template <class T, int U, bool BACK, bool DRAW, bool BIAS, bool EDGE>
 __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, int64_t e, int64_t advance, const Pack<T> (&in)[U],
                                              const Pack<T> (&y)[U], const float2 (&b)[kVec<T> / 2], float2 (&o)[U][kVec<T> / 2]) {
   constexpr int V = kVec<T>, H = V / 2;
+  constexpr bool MARK = !BACK && BIAS && sizeof(T) == 2;       // the ReLU follows at the store
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     unpack<T>(in[u], o[u]);
@@ -488,28 +489,22 @@ __device__ __forceinline__ void drop_vectors(const DropArgs& a, uint64_t step, i
 #pragma unroll
         for (int t = 0; t < H; ++t) o[u][t] = __fadd2_rn(o[u][t], b[t]);
       }
-      if (a.relu) {
+      if (!MARK && a.relu) {
 #pragma unroll
         for (int t = 0; t < H; ++t) o[u][t] = make_float2(relu_of(o[u][t].x), relu_of(o[u][t].y));
       }
     }
   }
-  scale_elements(o, a.drop.scale);
-  if constexpr (!BACK && BIAS && sizeof(T) == 2) {
-    if (a.relu && a.bf32) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int t = 0; t < H; ++t) o[u][t] = make_float2(marked<T>(o[u][t].x), marked<T>(o[u][t].y));
-    }
-  }
+  if constexpr (MARK) scaled<T>(o, a.drop.scale, a.relu);
+  else scale_elements(o, a.drop.scale);
   if constexpr (DRAW) {
+    const float dropped = MARK && a.relu ? -0.0f : 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint32_t words[V];
       draw_words<1, V, EDGE>(a.drop, step, e + u * advance, 0, words);
 #pragma unroll
-      for (int t = 0; t < H; ++t) o[u][t] = kept_of(a.drop, words + 2 * t, o[u][t]);
+      for (int t = 0; t < H; ++t) o[u][t] = kept_of(a.drop, words + 2 * t, o[u][t], dropped);
     }
   }
 }
@@ -598,7 +593,7 @@ __global__ void __launch_bounds__(256, drop_row_blocks<T, BACK && !DRAW, EDGE>()
 #pragma unroll
             for (int t = 0; t < V / 2; ++t) acc[t] = __fadd2_rn(acc[t], o[u][t]);
           }
-          if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o[u]);
+          if (a.out != nullptr) store_vec<T, EDGE>(reinterpret_cast<T*>(a.out) + (r + u * stride) * a.ldo, c, a.dim, o[u], !BACK && a.relu);
         }
     }
   }
@@ -633,7 +628,8 @@ template <class T, bool BACK>
 __global__ void __launch_bounds__(256, 4) dropout_any_kernel(const __grid_constant__ DropArgs a, int whole) {
   constexpr int U = 2;
   const uint64_t step = step_of(a.drop);
-  const bool two = BACK && a.relu, draw = a.drop.on && !two;
+  constexpr bool MARK = !BACK && sizeof(T) == 2;
+  const bool two = BACK && a.relu, draw = a.drop.on && !two, mark = MARK && a.relu;
   const int64_t n = a.rows * a.dim, ahead = a.drop.first & 3;         // element 0 is number `ahead` of its group
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -659,17 +655,29 @@ __global__ void __launch_bounds__(256, 4) dropout_any_kernel(const __grid_consta
       float z = to_float(in[t]);
       if constexpr (BACK) {
         if (two && !passed(y[t])) z = 0.0f;
+        z *= a.drop.scale;
       } else {
         if (a.bias != nullptr) z += vector_at<T>(a.bias, a.bf32, c);
-        if (a.relu) z = relu_of(z);
+        if (!MARK && a.relu) z = relu_of(z);
+        z = __fmaf_rn(z, a.drop.scale, mark ? -kLeast : -0.0f);
       }
-      z *= a.drop.scale;
-      if (!BACK && a.relu) z = marked<T>(z);
-      out[t] = from_float<T>(draw && words[t] <= a.drop.last ? 0.0f : z);
-      if (!(full && (whole & 4))) reinterpret_cast<T*>(a.out)[r * a.ldo + c] = out[t];
+      out[t] = from_float<T>(draw && words[t] <= a.drop.last ? (mark ? -0.0f : 0.0f) : z);
+      if (!(full && (whole & 4))) {
+        if constexpr (MARK) {
+          if (mark) out[t] = relu_marked_one(out[t]);
+        }
+        reinterpret_cast<T*>(a.out)[r * a.ldo + c] = out[t];
+      }
       if (++c == a.dim) {
         c = 0;
         ++r;
+      }
+    }
+    if constexpr (MARK) {
+      if (mark && full && (whole & 4)) {
+        uint32_t* pair = reinterpret_cast<uint32_t*>(out);
+        pair[0] = relu_marked<T>(pair[0]);
+        pair[1] = relu_marked<T>(pair[1]);
       }
     }
     if (full && (whole & 4)) four_copy(reinterpret_cast<T*>(a.out) + i0, out);

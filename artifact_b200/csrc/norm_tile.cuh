@@ -119,8 +119,21 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
     }
     if (ODD && c0 < 0) v[0].x = 0.0f;
   };
+  constexpr bool kMark = MODE == kDropForward && sizeof(T) == 2;   // the ReLU follows the rounding
   const auto write = [&](T* row, int j, float2 v) {
     const int c = c0 + 2 * L * j;
+    if constexpr (kMark) {
+      if (a.relu) {
+        alignas(4) T two[2];
+        pack_two(two, v);
+        uint32_t* pair = reinterpret_cast<uint32_t*>(two);
+        *pair = relu_marked<T>(*pair);
+        if (ODD && j == 0 && c < 0) row[0] = two[1];
+        else if (j < kSure || c + 1 < dim) *reinterpret_cast<uint32_t*>(row + c) = *pair;
+        else if (ODD && c < dim) row[c] = two[0];
+        return;
+      }
+    }
     if (ODD && j == 0 && c < 0) row[0] = from_float<T>(v.y);
     else if (j < kSure || c + 1 < dim) pack_two(row + c, v);
     else if (ODD && c < dim) row[c] = from_float<T>(v.x);
@@ -257,16 +270,16 @@ __global__ void __launch_bounds__(256, tile_blocks<MODE, E>()) norm_tile_kernel(
         } else {
 #pragma unroll
           for (int j = 0; j < P; ++j) v[j] = __fadd2_rn(v[j], b[j]);
-          if (a.relu) {
+          if (!kMark && a.relu) {
 #pragma unroll
             for (int j = 0; j < P; ++j) v[j] = make_float2(relu_of(v[j].x), relu_of(v[j].y));
           }
         }
+        const float least = kMark && a.relu ? -kLeast : -0.0f;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          v[j] = __fmul2_rn(v[j], both(a.drop.scale));
+          v[j] = __ffma2_rn(v[j], both(a.drop.scale), both(least));
           if constexpr (kBack) ab[j] = __fadd2_rn(ab[j], v[j]);
-          if (!kBack && sizeof(T) == 2 && a.relu && a.f32) v[j] = make_float2(marked<T>(v[j].x), marked<T>(v[j].y));
           write(pa, j, v[j]);
         }
       }
