@@ -52,9 +52,9 @@ inline int column_blocks_cap(int64_t rows, int dim) {
   return (int)std::min<int64_t>(cap, (std::max<int64_t>(rows, 1) + 7) / 8 * 8);
 }
 
-// Whether a 16-byte vector of `vec` elements whose first is in column c of a row ends in the matrix, with `behind` rows after its own.  A vector
-// that passes the end of its row reaches up to vec - 1 elements further: into rows of one column and more that many rows follow.
-__host__ __device__ inline bool ends_in_matrix(int64_t behind, int c, int dim, int vec) { return c + vec <= dim || behind >= vec; }
+// Whether a 16-byte vector of `vec` elements whose first is in column c of row r ends in the matrix.  One that passes the end of its row
+// reaches up to vec - 1 elements further: into rows of one column and more, of which that many follow.
+__host__ __device__ inline bool ends_in_matrix(int64_t r, int64_t rows, int c, int dim, int vec) { return c + vec <= dim || r < rows - vec; }
 
 // The tile kernels (norm_tile.cuh).
 enum TileMode { kNormForward, kNormForwardHidden, kNormBackward, kNormBackwardHidden, kDropForward, kDropBackward };

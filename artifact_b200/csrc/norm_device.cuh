@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <initializer_list>
 #include <type_traits>
 
@@ -44,11 +45,11 @@ union Pack {
   __device__ Pack() {}
 };
 
-// Columns [c, c + VEC) of a row, c + VEC > 0, with `behind` rows after it.  Partial vectors hold what the 16 bytes hold, the neighbouring
+// Columns [c, c + VEC) of row r, c + VEC > 0.  Partial vectors hold what the 16 bytes hold, the neighbouring
 // row's elements or what precedes the matrix in its allocation; behind the end of the matrix nothing is read.
 template <class T, bool EDGE>
-__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim, int64_t behind) {
-  if (!EDGE || ends_in_matrix(behind, c, dim, kVec<T>)) {
+__device__ __forceinline__ void load_vec(Pack<T>& out, const T* row, int c, int dim, int64_t r, int64_t rows) {
+  if (!EDGE || ends_in_matrix(r, rows, c, dim, kVec<T>)) {
     out.raw = *reinterpret_cast<const uint4*>(row + c);
   } else {
 #pragma unroll
@@ -152,17 +153,19 @@ struct Ring {
   }
 };
 
-// 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place; of zero and infinity the approximation is the value,
-// and the step would make a NaN of it
+// 1 / sqrt(v): the approximation and one Newton step, within a unit in the last place; 0 of infinity, whose product with the
+// approximation would be a NaN
 __device__ __forceinline__ float rsqrt_of(float v) {
   const float r = rsqrtf(v);
-  return v > 0.0f && v < INFINITY ? __fmaf_rn(0.5f * r, __fmaf_rn(-(v * r), r, 1.0f), r) : r;
+  return __fmaf_rn(0.5f * r, __fmaf_rn(-(fminf(v, FLT_MAX) * r), r, 1.0f), r);
 }
 
 // The variance from a row's mean square deviation from a first mean that is `off` from the mean.  Where the squares pass the range of
-// 32 bits it is infinite: the row then has rstd 0 and becomes its bias.
+// 32 bits it is infinite: the row then has rstd 0 and becomes its bias.  (`square` is no less than off^2, so an `off` whose square is out of
+// range stands beside an infinite one: it may be any smaller number.)
 __device__ __forceinline__ float variance_of(float square, float off) {
-  return square < INFINITY ? fmaxf(__fmaf_rn(-off, off, square), 0.0f) : square;
+  off = fminf(fabsf(off), 0x1.fffffep63f);
+  return fmaxf(__fmaf_rn(-off, off, square), 0.0f);
 }
 
 // Two elements at a time: the f32x2 instructions of sm_100, each half rounded like the scalar one.
@@ -250,7 +253,8 @@ __device__ __forceinline__ float relu_of(float z) {
 // and still round to a zero of a 16-bit type.  That zero is stored with its sign set; every other zero is +0.  On the way the signs are
 // the other way round, because the rounding then keeps them apart by itself: what is not positive or dropped is negative or -0
 // (`scaled`: an exact zero is taken down by the least number there is), what is positive is +0 at least.  So two elements cost the ReLU
-// as a maximum with -0, a comparison and an exclusive or (1000000x64 bf16: 77 us forward; choosing in 32 bits 84, without any 73).
+// as a maximum with -0, a comparison and an exclusive or (1000000x64 bf16: 67 us forward; choosing in
+// 32 bits 84; without marks, the ReLU in 32 bits, 73).
 constexpr float kLeast = 0x1p-149f;
 template <class T, int C, int H>
 __device__ __forceinline__ void scaled(float2 (&v)[C][H], float f, bool relu) {

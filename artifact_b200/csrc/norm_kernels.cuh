@@ -360,9 +360,10 @@ __global__ void __launch_bounds__(256) join_columns_kernel(const float* partial,
   const int x = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + x;
   float sum = 0.0f;
+  partial += i;
   if (i < width) {
 #pragma unroll 8
-    for (int k = run; k < blocks; k += 8) sum += partial[k * width + i];
+    for (int k = run; k < blocks; k += 8) sum += partial[k * width];
   }
   part[run][x] = sum;
   __syncthreads();
@@ -579,9 +580,8 @@ __global__ void __launch_bounds__(256, drop_row_blocks<T, BACK && !DRAW, EDGE>()
       for (int u = 0; u < U; ++u) {
         in[u].raw = yy[u].raw = make_uint4(0, 0, 0, 0);
         if (r + u * stride < a.rows) {
-          const int64_t behind = a.rows - 1 - (r + u * stride);
-          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim, behind);
-          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim, behind);
+          load_vec<T, EDGE>(in[u], reinterpret_cast<const T*>(a.x) + (r + u * stride) * a.ldx, c, a.dim, r + u * stride, a.rows);
+          if (two) load_vec<T, EDGE>(yy[u], reinterpret_cast<const T*>(a.y) + (r + u * stride) * a.ldy, c, a.dim, r + u * stride, a.rows);
         }
       }
       float2 o[U][V / 2];

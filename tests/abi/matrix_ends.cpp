@@ -15,7 +15,7 @@ int main() {
               const int first = r * ld, shift = (start + (rows > 1 ? first : 0)) % vec, end = (rows - 1) * ld + dim;
               for (int c = -shift; c < dim; c += vec) {
                 const bool inside = first + c + vec <= end;
-                if (!rof::ends_in_matrix(rows - 1 - r, c, dim, vec)) held += inside && rows - 1 - r >= vec;
+                if (!rof::ends_in_matrix(r, rows, c, dim, vec)) held += inside && rows - 1 - r >= vec;
                 else ++(inside ? right : wrong);
               }
             }
