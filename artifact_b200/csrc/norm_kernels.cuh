@@ -10,11 +10,14 @@
 // which are cleared after the load and not written.  s has period VEC in the row number, and the groups advance by a multiple of
 // VEC rows, so a thread's columns never change.  The inputs of a call must share s; an output that lies differently is
 // written through shared memory.  What is left — inputs that lie differently, rows of more than 8,192 columns — runs on the
-// *_plain kernels.  (Odd widths up to 511 in contiguous matrices: norm_tile.cuh.)
+// *_plain kernels.  (Contiguous matrices of up to 511 columns whose rows are not whole vectors: norm_tile.cuh.)
 //
 // Measured on B200, of the measured copy bandwidth (6,460 GB/s; every matrix read or written once per pass): layer norm
-// 2449029x256 fp32 forward 764 us (102 %), back 1,180 us (99 %); 232965x602 fp32 177 us (98 %), 278 us (94 %); 16384x4096
-// bf16 52 us (81 %), 87 us (71 %: a block per row and few warps to cover its two sums).
+// 2449029x256 fp32 forward 764 us (102 %), back 1,180 us (99 %); 232965x602 fp32 178 us (98 %), 287 us (91 %); 16384x4096
+// bf16 52 us (80 %), 89 us (70 %: a block per row and few warps to cover its two sums).  With the ReLU and the generator in 16 bits neither
+// DRAM nor the issue slots are full (1000000x64 bf16: 74 us, 53 %; 103 us, 58 %): two blocks of 256 threads an SM do not cover the
+// row's chain of sums and rounds.  Padded rows beside contiguous ones: 200000x301 fp32 80 and 130 us (93 and 86 %), 1000000x47
+// bf16 100 and 105 us (29 and 41 %).  The *_plain kernels: 30000x10000 fp32 1,056 and 2,107 us (35 and 26 %).
 #pragma once
 #include "norm_device.cuh"
 
@@ -39,12 +42,14 @@ constexpr int wide_threads() { return C * kVec<T> <= 16 ? 512 : 256; }
 // The forward pass runs two blocks of 256 threads per SM and no more: with the rings, 512 threads keep enough in flight, and more of
 // them only mix their reads and writes more finely (2449029x256 fp32: 760 us with two, 834 with three, 956 with one).
 constexpr int kForwardBlocks = 2;
-// Blocks of 256 threads per SM that the register allocation aims at: in the backward pass as many as leave nothing spilled; in the
-// forward pass two, where 32 elements a thread with the generator and partial vectors would spill 400 bytes one (200000x1001
-// fp32: 351 us, 433 with two; 20 elements, 300000x602: 264 us with two, 357 with one).
+// Blocks of 256 threads per SM that the register allocation aims at.  Backward: as many as spill at most 8 bytes (rows of a block have
+// registers of their own, wide_threads(), and up to 92).  Forward: two; one for 32 elements a thread with the generator and partial vectors,
+// which would spill 400 bytes with two (200000x1001 fp32: 351 us, 433 with two).  At 24 elements two blocks spill 120 bytes and are
+// faster all the same (300000x601 bf16 331 us, 394 with one; with padded rows, 200 bytes, 436 and 488, but 500000x300 314 and 296); at 20
+// they spill 8 (60 with padded rows; 300000x602 fp32 261 and 352).
 template <class T, int C, bool HIDDEN, bool EDGE>
 constexpr int forward_blocks() { return HIDDEN && EDGE && C * kVec<T> > 24 ? 1 : kForwardBlocks; }
-template <class T, int C, bool HIDDEN, bool EDGE>
+template <class T, int C, bool HIDDEN>
 constexpr int backward_blocks() { return C * kVec<T> <= 8 ? (HIDDEN ? 2 : 3) : C * kVec<T> <= (HIDDEN ? 8 : 16) ? 2 : 1; }
 // Slots of the rings.  In the forward pass 32-bit rows do best with little in flight (2 slots of 64 bytes a thread and more: 65536x2048 172 us
 // against 191 with 3), 16-bit rows, which take more instructions a byte, with more (16384x4096 51 us with 4, 54 with 3).
@@ -233,7 +238,7 @@ __device__ __forceinline__ void store_columns(const float2 (&acc)[C][kVec<T> / 2
 
 // dx of every row, and per block the sums over its rows of dz h and dz: partial[block][2][dim]
 template <class T, int L, int C, bool HIDDEN, int LAYOUT>
-__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN, LAYOUT != kWhole>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(L == 0 ? wide_threads<T, C>() : 256, L == 0 ? 1 : backward_blocks<T, C, HIDDEN>()) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int V = kVec<T>, H = V / 2;
   constexpr bool EDGE = LAYOUT != kWhole;
   __shared__ float buf[2][32];
@@ -741,8 +746,14 @@ bool wide_rows(int vectors, F&& f) {
 }
 
 // Group width L and vectors per lane C for rows of `vectors` vectors -> f.template operator()<L, C>(block threads).  The
-// fewest lanes whose registers hold the row: they have the most bytes in flight each and the fewest steps in the row's sums.
-// The backward pass through a ReLU or a dropout also keeps the biases and the words, and gets by with fewer elements a thread.
+// fewest lanes whose registers hold the row: they have the most bytes in flight each and the fewest steps in the row's sums.  How much a
+// lane holds: in 32 bits up to 5 vectors (20 elements: weights, biases and sums beside them leave two blocks an SM), a full warp up to 8 in
+// the forward pass, where the next choice is a block per row; in 16 bits up to 3 (24 elements), a full warp up to 4 in the backward pass
+// (65536x1024 bf16: 73 us, 87 with a block per row).  Back through a ReLU or a dropout, with biases and words as well, up to 3 vectors in 32
+// bits and one in 16, a full warp 5 and 2.  Wider rows have a block each, and a thread of it what wide_threads() has registers for (16-bit
+// rows of 97 to 256 vectors forward: 16 elements; 32 would leave a block one or two warps).  So a block owns a row above 1,024
+// columns (fp32 forward, 16-bit backward), 768 (16-bit forward), 640 (fp32 backward, with a ReLU or a dropout too) and 512 (16-bit
+// backward with one).
 enum Pass { kForward, kBackward, kBackwardHidden };
 template <class T, Pass PASS, class F>
 bool by_width(int vectors, F&& f) {

@@ -1,4 +1,4 @@
-// Layer norm and dropout for contiguous matrices whose rows are not whole 16-byte vectors (odd widths up to 512).
+// Layer norm and dropout for contiguous matrices of up to 511 columns whose rows are not whole 16-byte vectors.
 //
 // Rows like these share their 16-byte vectors with their neighbours, and a thread that owns vectors of one row spends more
 // instructions on the row's two ends than on its middle (47 columns in bf16: 35 instructions an element).  But R = 256 / L rows of a
@@ -8,10 +8,11 @@
 // 16-byte stores.  Dropout is decided on the run too, where four neighbours share a call of the generator: the forward
 // pass clears what is dropped on the way out, the backward pass in dy on the way in.
 //
-// Bound by HBM in 32 bits (2449029x47 layer norm: 160 us forward, 242 us back, 88 % of the measured copy bandwidth), by instructions in
-// 16 (107 and 146 us, 67 and 73 %: 24 instructions an element keep 71 % of the issue slots busy) and with the generator
-// (ReLU and dropout, fp32: 203 and 278 us, 70 and 77 %).  L and E follow the width: the fewest lanes whose registers hold the row
-// (half as many elements a thread: 205 us instead of 171 forward in bf16).
+// Measured, of the measured copy bandwidth: 2449029x47 layer norm fp32 160 us forward, 242 us back (88 %: HBM), bf16 107 and 148 us (66 and
+// 72 %); with ReLU and dropout fp32 203 and 281 us (70 and 76 %), bf16 223 and 254 us (32 and 42 %).  The forward pass in 16 bits keeps
+// 71 % of the issue slots busy (24 instructions an element); the others are short of both limits, with 24 to 34 % of the warps and two
+// barriers a tile.  L and E follow the width: the fewest lanes whose registers hold the row (half as many elements a thread: 205 us
+// instead of 171 forward in bf16).
 #pragma once
 #include <type_traits>
 
@@ -38,10 +39,10 @@ __device__ __forceinline__ void clear_dropped(const Drop& d, const uint32_t* w, 
   }
 }
 
-// Blocks per SM that the register allocation aims at: as many as leave nothing spilled.
+// Blocks per SM that the register allocation aims at: as many as spill at most 16 bytes.
 template <int MODE, int E>
 constexpr int tile_blocks() {
-  return MODE == kNormBackwardHidden ? (E <= 4 ? 3 : 2) : MODE == kNormBackward ? (E <= 8 ? 3 : 2) : MODE == kNormForwardHidden ? (E <= 8 ? 3 : E <= 12 ? 3 : 2) : (E <= 8 ? 4 : 3);
+  return MODE == kNormBackwardHidden ? (E <= 4 ? 3 : 2) : MODE == kNormBackward ? (E <= 8 ? 3 : 2) : MODE == kNormForwardHidden ? (E <= 12 ? 3 : 2) : (E <= 8 ? 4 : 3);
 }
 
 // E elements per thread.  Pair j of lane i holds columns c, c + 1 with c = 2 (i + L j) - s: s = 1 for the odd rows of an odd width (ODD),
